@@ -142,6 +142,70 @@ MAXSIM_API int maxsim_b200_copy_valid_rows(const void* src, int src_is_host,
                                            int64_t row_bytes, void* stream);
 MAXSIM_API int maxsim_b200_topk_rows(const float* scores, int64_t rows, int64_t cols, int64_t k,
                                      float* values, int64_t* indices, void* stream);
+/* sample_rows: n candidates of each score row, drawn without replacement from
+ * given random numbers (no reference counterpart).  scores and uniforms are
+ * [rows, cols] float, rows score_stride / uniform_stride elements apart.  An
+ * entry that is NaN or -inf is no candidate; with a_i = (s_i - max s) /
+ * temperature (0 for the best, an infinite one included) a candidate weighs
+ * exp(a_i), and one with a_i < -700 is none.  In the order score descending,
+ * index ascending the filters keep the first top_k (<= 0: all), of those the
+ * ones before which less than top_p of their weight lies (outside (0, 1): all),
+ * and the ones that weigh at least min_p of the best (outside (0, 1]: all).
+ * Drawn are the n largest of a_i - log(-log(uniform_i)) among the kept, largest first, equal
+ * ones by ascending index; a uniform outside [0, 1] leaves its candidate out.
+ * indices [rows, n] int64 (-1 when fewer are left) and probabilities [rows, n]
+ * float: the drawn candidate's share of the kept weight (0 where the index is
+ * -1).  Each of the four parameters is a value, or one per row where its _rows
+ * array [rows] on the device is not NULL; a row whose temperature is not > 0 draws nothing.
+ * cols <= 2^20, n <= 1024. */
+MAXSIM_API int maxsim_b200_sample_rows(const float* scores, int64_t score_stride,
+                                       const float* uniforms, int64_t uniform_stride,
+                                       int64_t rows, int64_t cols, int64_t n,
+                                       double temperature, const float* temperature_rows,
+                                       int64_t top_k, const int32_t* top_k_rows,
+                                       double top_p, const float* top_p_rows,
+                                       double min_p, const float* min_p_rows,
+                                       int64_t* indices, float* probabilities, void* stream);
+
+/* Row normalisation between an encoder and the operators (no reference
+ * counterpart).  Token rows of `dim` elements of type `dtype` lie [n_segments,
+ * L_max]; row (n, j) starts n * segment_stride + j * row_stride elements into
+ * `tokens`.  offsets NULL: every row counts and is row n * L_max + j of the outputs.
+ * Otherwise [n_segments + 1] int32: row (n, j) counts for j < offsets[n+1] -
+ * offsets[n] and is row offsets[n] + j of the outputs; outputs have packed_rows rows,
+ * and rows at or beyond are never touched.
+ *   MAXSIM_NORM_LAYER: out = (x - mean) * rstd * weight + bias with rstd =
+ *     1 / sqrt(var + eps); weight and bias [dim] of type weight_dtype (`dtype`
+ *     or MAXSIM_F32), each may be NULL.  mean and rstd [packed_rows] float are
+ *     written for the backward pass, or both NULL.
+ *   MAXSIM_NORM_UNIT: out = x / max(|x|, eps); no weights, no statistics.
+ * The backward call takes grad [packed_rows, dim] of type `dtype` and writes
+ * those of grad_tokens [n_segments, L_max, dim] (contiguous, zero for rows that
+ * do not count), grad_weight and grad_bias [dim] that are not NULL.  grad_weight and
+ * grad_bias need a workspace of maxsim_b200_norm_rows_workspace bytes on the
+ * device, whose contents before and after the call do not matter; equal calls give equal
+ * bits.  At most 2^31 - 1 rows; eps >= 1e-30. */
+typedef enum maxsim_norm {
+  MAXSIM_NORM_LAYER = 0,
+  MAXSIM_NORM_UNIT = 1
+} maxsim_norm;
+MAXSIM_API int maxsim_b200_norm_rows(int norm, const void* tokens, int64_t segment_stride,
+                                     int64_t row_stride, const int32_t* offsets,
+                                     const void* weight, const void* bias, void* out,
+                                     float* mean, float* rstd, int64_t n_segments,
+                                     int64_t L_max, int64_t dim, int64_t packed_rows,
+                                     double eps, int dtype, int weight_dtype, void* stream);
+MAXSIM_API int64_t maxsim_b200_norm_rows_workspace(int64_t n_segments, int64_t L_max, int64_t dim);
+MAXSIM_API int maxsim_b200_norm_rows_backward(int norm, const void* grad, const void* tokens,
+                                              int64_t segment_stride, int64_t row_stride,
+                                              const int32_t* offsets, const void* weight,
+                                              const float* mean, const float* rstd,
+                                              void* grad_tokens, void* grad_weight,
+                                              void* grad_bias, void* workspace,
+                                              int64_t workspace_bytes, int64_t n_segments,
+                                              int64_t L_max, int64_t dim, int64_t packed_rows,
+                                              double eps, int dtype, int weight_dtype,
+                                              void* stream);
 
 /* ------------------------------------------------------------------------
  * Packed pair grids.

@@ -29,8 +29,9 @@ from . import _ops
 from . import _validate as _v
 from ._ops import device_status, ops
 from .graphed import GraphedContrastiveStep, GraphedShardedContrastiveStep
-from .layout import (pack_padded, rerank_order, rerank_topk, score_candidates_padded_from_host,
-                     unpack_packed)
+from .layout import (pack_padded, rerank_order, rerank_topk, sample_candidates,
+                     score_candidates_padded_from_host, unpack_packed)
+from .norms import layer_norm, pack_layer_norm, pack_unit_norm, unit_norm
 
 __all__ = [
     "score_pairs_packed", "score_pairs_packed_with_argmax", "score_pairs_packed_train",
@@ -40,7 +41,8 @@ __all__ = [
     "score_padded", "score_padded_with_argmax", "score_padded_train",
     "score_packed", "score_packed_with_argmax", "score_packed_train",
     "lengths_from_prefix_mask", "contrastive_loss",
-    "pack_padded", "unpack_packed", "rerank_topk", "rerank_order",
+    "pack_padded", "unpack_packed", "rerank_topk", "rerank_order", "sample_candidates",
+    "layer_norm", "pack_layer_norm", "unit_norm", "pack_unit_norm",
     "score_candidates_padded_from_host", "GraphedContrastiveStep", "GraphedShardedContrastiveStep", "device_status",
 ]
 

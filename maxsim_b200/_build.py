@@ -13,6 +13,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -20,11 +22,11 @@ CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libmaxsim_b200.so"
 STAMP_PATH = PKG_DIR / "libmaxsim_b200.stamp"
 
-SOURCES = ["abi.cu"]
+SOURCES = ["abi.cu", "steps.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "--shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
     "-Xcompiler", "-fvisibility=hidden",
 ]
 
@@ -36,7 +38,7 @@ def _find_nvcc() -> str | None:
 
 def source_digest() -> str:
     h = hashlib.sha256()
-    files = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh"))
+    files = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
     files.append(PKG_DIR.parent / "include" / "maxsim_b200.h")
     for f in files:
         h.update(f.name.encode())
@@ -65,16 +67,21 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if not force and is_current():
             return LIB_PATH
         tmp = LIB_PATH.with_suffix(f".so.tmp{os.getpid()}")
-        cmd = [nvcc, *NVCC_FLAGS]
-        if verbose:
-            cmd += ["-Xptxas", "-v"]
-        cmd += ["-o", str(tmp)] + [str(CSRC / s) for s in SOURCES]
-        proc = subprocess.run(cmd, capture_output=True, text=True)
-        if proc.returncode != 0:
+        with tempfile.TemporaryDirectory() as work:
+            objects = [str(Path(work) / f"{Path(s).stem}.o") for s in SOURCES]
+            cmds = [[nvcc, *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-c", "-o", o, str(CSRC / s)]
+                    for s, o in zip(SOURCES, objects)]
+            with ThreadPoolExecutor(len(cmds)) as pool:  # one compiler per source, side by side
+                procs = list(pool.map(lambda c: subprocess.run(c, capture_output=True, text=True), cmds))
+            if all(p.returncode == 0 for p in procs):
+                procs.append(subprocess.run([nvcc, *NVCC_FLAGS, "--shared", "-o", str(tmp), *objects],
+                                            capture_output=True, text=True))
+        failed = [p for p in procs if p.returncode != 0]
+        if failed:
             tmp.unlink(missing_ok=True)
-            raise RuntimeError("nvcc failed:\n" + proc.stdout + proc.stderr)
+            raise RuntimeError("nvcc failed:\n" + "".join(p.stdout + p.stderr for p in failed))
         if verbose:
-            sys.stderr.write(proc.stderr)
+            sys.stderr.write("".join(p.stderr for p in procs))
         os.replace(tmp, LIB_PATH)
         STAMP_PATH.write_text(source_digest() + "\n")
     return LIB_PATH

@@ -32,6 +32,7 @@ _DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _lib = None
 
 _I64 = c_int64
+_F64 = ctypes.c_double
 _P = c_void_p
 
 _SIGNATURES = {
@@ -47,6 +48,12 @@ _SIGNATURES = {
     "maxsim_b200_pack_rows": (c_int, [_P] * 3 + [_I64] * 4 + [_P]),
     "maxsim_b200_unpack_rows": (c_int, [_P] * 3 + [_I64] * 4 + [_P]),
     "maxsim_b200_topk_rows": (c_int, [_P] + [_I64] * 3 + [_P] * 3),
+    "maxsim_b200_sample_rows": (c_int, [_P, _I64, _P, _I64, _I64, _I64, _I64, _F64, _P, _I64, _P, _F64, _P, _F64, _P]
+                                + [_P] * 3),
+    "maxsim_b200_norm_rows": (c_int, [c_int, _P, _I64, _I64] + [_P] * 6 + [_I64] * 4 + [_F64, c_int, c_int, _P]),
+    "maxsim_b200_norm_rows_workspace": (c_int64, [_I64] * 3),
+    "maxsim_b200_norm_rows_backward": (c_int, [c_int, _P, _P, _I64, _I64] + [_P] * 8 + [_I64] * 5
+                                       + [_F64, c_int, c_int, _P]),
     "maxsim_b200_copy_valid_rows": (c_int, [_P, c_int, _P, _P] + [_I64] * 3 + [_P]),
     "maxsim_b200_group_pairs": (c_int, [_P, _I64, _I64, _P, _P, _P]),
     "maxsim_b200_group_pairs_static": (c_int, [_P, _I64, _I64, _P, _P]),
@@ -271,6 +278,77 @@ def topk_rows(scores: torch.Tensor, k: int):
     return values, indices
 
 
+def sample_rows(scores: torch.Tensor, uniforms: torch.Tensor, n: int, temperature, top_k, top_p, min_p):
+    """``scores`` / ``uniforms [rows, cols]`` fp32 with a contiguous last
+    dimension -> ``(indices [rows, n] int64, probabilities [rows, n] fp32)``.
+    Each of the four parameters is a number or a ``[rows]`` tensor (fp32, int32
+    for ``top_k``) on the same device; ``top_k`` 0, ``top_p`` 1 and ``min_p`` 0
+    filter nothing."""
+    params = []
+    for value in (temperature, top_k, top_p, min_p):
+        params += [0, value] if isinstance(value, torch.Tensor) else [value, None]
+    dev = _require_cuda(scores, uniforms, *(t for t in params[1::2] if t is not None))
+    rows, cols = scores.shape
+    indices = torch.empty((rows, int(n)), dtype=torch.int64, device=dev)
+    probabilities = torch.empty((rows, int(n)), dtype=torch.float32, device=dev)
+    for i in (1, 3, 5, 7):
+        params[i] = 0 if params[i] is None else _ptr(params[i])
+    with _on_device(dev):
+        rc = load_library().maxsim_b200_sample_rows(
+            _ptr(scores), scores.stride(0), _ptr(uniforms), uniforms.stride(0), rows, cols, int(n),
+            *params, _ptr(indices), _ptr(probabilities), _stream_ptr())
+    _check(rc, "maxsim_b200_sample_rows")
+    return indices, probabilities
+
+
+NORM_LAYER, NORM_UNIT = 0, 1
+
+
+def norm_rows(kind: int, tokens: torch.Tensor, strides, shape, offsets, packed_rows: int, weight, bias,
+              eps: float, want_stats: bool):
+    """Normalise the rows of ``tokens``: ``shape`` is ``(n_segments, L_max, dim)``
+    and ``strides`` the element strides of its first two dimensions (the last
+    is contiguous).  With ``offsets [n_segments + 1]`` int32 the rows that count
+    are written back to back.  Returns ``(out [packed_rows, dim], mean, rstd)``;
+    the statistics are None unless asked for (layer norm only)."""
+    dev = _require_cuda(*(t for t in (tokens, offsets, weight, bias) if t is not None))
+    n, L, dim = shape
+    out = torch.empty((packed_rows, dim), dtype=tokens.dtype, device=dev)
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = torch.empty((2, packed_rows), dtype=torch.float32, device=dev)
+    with _on_device(dev):
+        rc = load_library().maxsim_b200_norm_rows(
+            kind, _ptr(tokens), strides[0], strides[1], offsets.data_ptr() if offsets is not None else 0,
+            _opt(weight), _opt(bias), _ptr(out), _opt(mean), _opt(rstd), n, L, dim, packed_rows, eps,
+            _code(tokens), _code(weight) if weight is not None else 0, _stream_ptr())
+    _check(rc, "maxsim_b200_norm_rows")
+    return out, mean, rstd
+
+
+def norm_rows_backward(kind: int, grad: torch.Tensor, tokens: torch.Tensor, strides, shape, offsets, weight,
+                       mean, rstd, eps: float, want_tokens: bool, want_weight: bool, want_bias: bool):
+    """The gradients of :func:`norm_rows` that are wanted, else None:
+    ``(grad_tokens [n_segments, L_max, dim], grad_weight [dim], grad_bias [dim])``."""
+    dev = _require_cuda(*(t for t in (tokens, grad, offsets, weight, mean, rstd) if t is not None))
+    n, L, dim = shape
+    lib = load_library()
+    dx = torch.empty(shape, dtype=tokens.dtype, device=dev) if want_tokens else None
+    dw = torch.empty((dim,), dtype=weight.dtype, device=dev) if want_weight else None
+    db = torch.empty((dim,), dtype=weight.dtype, device=dev) if want_bias else None
+    with _on_device(dev):
+        work = None
+        if want_weight or want_bias:
+            work = torch.empty((lib.maxsim_b200_norm_rows_workspace(n, L, dim),), dtype=torch.uint8, device=dev)
+        rc = lib.maxsim_b200_norm_rows_backward(
+            kind, _ptr(grad), _ptr(tokens), strides[0], strides[1],
+            offsets.data_ptr() if offsets is not None else 0, _opt(weight), _opt(mean), _opt(rstd), _opt(dx),
+            _opt(dw), _opt(db), _opt(work), work.numel() if work is not None else 0, n, L, dim, grad.shape[0], eps,
+            _code(tokens), _code(weight) if weight is not None else 0, _stream_ptr())
+    _check(rc, "maxsim_b200_norm_rows_backward")
+    return dx, dw, db
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _exchange_device = getattr(torch.cuda, "_exchange_device", None)
 
@@ -314,6 +392,10 @@ class _on_device:
 
 def _ptr(t: torch.Tensor) -> int:
     return t.data_ptr() if t.numel() else 0
+
+
+def _opt(t) -> int:
+    return _ptr(t) if t is not None else 0
 
 
 def _require_cuda(*tensors: torch.Tensor) -> torch.device:

@@ -14,17 +14,19 @@
 #include "fwd_tc05_any.cuh"
 #include "fwd_tc05_doc.cuh"
 #include "group.cuh"
+#include "host.h"
 #include "layout_stats.cuh"
 #include "loss.cuh"
 #include "pack.cuh"
 
 namespace maxsim {
 
+// The helpers of host.h: this file defines what the library keeps per process.
 namespace {
-
 thread_local std::string t_last_error;
 std::atomic<int64_t> g_launches{0};
 std::atomic<int> g_forward_path{0};
+}  // namespace
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -36,23 +38,12 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-#define MAXSIM_CUDA(expr)                                                         \
-  do {                                                                            \
-    cudaError_t e_ = (expr);                                                      \
-    if (e_ != cudaSuccess)                                                        \
-      return fail(MAXSIM_ECUDA, "%s failed: %s", #expr, cudaGetErrorString(e_)); \
-  } while (0)
-
 int launch_check(const char* what) {
   g_launches.fetch_add(1, std::memory_order_relaxed);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(MAXSIM_ECUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
   return MAXSIM_OK;
 }
-
-// Per-device caches below are written with the same value by every thread that
-// races on them, through atomics, so concurrent first calls are harmless.
-constexpr int kMaxDevices = 64;
 
 int sm_count() {
   static std::atomic<int> cached[kMaxDevices];
@@ -66,27 +57,13 @@ int sm_count() {
   return n;
 }
 
-// Opt a kernel in to `smem` bytes of dynamic shared memory, once per device.
-template <typename Kernel>
-int ensure_smem(Kernel kern, size_t smem, std::atomic<unsigned char>* done) {
-  int dev = 0;
-  MAXSIM_CUDA(cudaGetDevice(&dev));
-  const bool track = dev >= 0 && dev < kMaxDevices;
-  if (track && done[dev].load(std::memory_order_acquire)) return MAXSIM_OK;
-  MAXSIM_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  if (track) done[dev].store(1, std::memory_order_release);
-  return MAXSIM_OK;
-}
+namespace {
 
 // Mean document length up to which contrastive argmax launches tile every
 // document on its own.  Measured on 1024 x 1024 pairs, bf16, per-document tiles
 // against boundary-agnostic ones: 32-256 tokens 1.43 / 1.77 ms, 64-512 tokens
 // (mean 288) 2.43 / 2.56 ms, 300-1000 tokens 4.9-5.4 / 4.9-5.0 ms.
 constexpr int64_t kPerDocMaxMean = 320;
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-bool valid_dtype(int dtype) { return dtype == MAXSIM_F32 || dtype == MAXSIM_F16 || dtype == MAXSIM_BF16; }
 
 // ---------------------------------------------------------------------------
 // Forward dispatch

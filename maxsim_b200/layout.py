@@ -13,6 +13,8 @@ host, and rank with ``scores.argsort(dim=1, descending=True)``
   padding; differentiable;
 * :func:`rerank_topk` -- the ``k`` best candidates of every row of a score
   matrix, best first, equal scores by ascending candidate index;
+* :func:`sample_candidates` -- candidates drawn from every row by temperature,
+  top-k, top-p and min-p (hard negatives), from given random numbers;
 * :func:`score_candidates_padded_from_host` -- rerank a padded batch that
   lives in pinned host memory: a kernel reads only the valid token rows over
   PCIe (a padded batch is about one third padding), the scores go back to the
@@ -21,6 +23,7 @@ host, and rank with ``scores.argsort(dim=1, descending=True)``
 
 from __future__ import annotations
 
+from operator import index
 from typing import Optional, Tuple
 
 import torch
@@ -28,7 +31,7 @@ import torch
 from . import _ops
 from . import _validate as _v
 
-__all__ = ["pack_padded", "unpack_packed", "rerank_topk", "rerank_order",
+__all__ = ["pack_padded", "unpack_packed", "rerank_topk", "rerank_order", "sample_candidates",
            "score_candidates_padded_from_host"]
 
 _eager = torch.compiler.disable
@@ -60,26 +63,10 @@ class _UnpackFn(torch.autograd.Function):
         return _ops.pack_rows(grad_padded, offsets, ctx.rows), None, None
 
 
-@_eager
-def pack_padded(padded: torch.Tensor, lengths: torch.Tensor, *,
-                total_tokens: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Pack ``padded [N, L_max, D]`` (CUDA, any dtype) by prefix ``lengths [N]``.
-
-    Returns ``(packed [T, D], offsets [N+1] int32)`` ready for
-    ``score_contrastive*`` (documents) or ``score_pairs_packed*``.
-
-    ``lengths`` may live on the host or on the device.  On the host the offsets
-    are built there and nothing synchronises.  On the device a scan kernel
-    builds them; ``T`` is then read back (one synchronisation) unless the
-    caller passes ``total_tokens``, in which case nothing synchronises and the
-    value is trusted to equal ``lengths.sum()`` (rows beyond it are dropped,
-    never written out of bounds).
-
-    Raises ``ValueError`` for a shape mismatch or, when the lengths are visible
-    to the host, a length outside ``(0, L_max]``.
-    """
-    if padded.dim() < 2:
-        raise ValueError(f"padded must be at least 2-D [N, L_max, ...]; got shape {tuple(padded.shape)}")
+def packed_offsets(padded: torch.Tensor, lengths: torch.Tensor, total_tokens: Optional[int]):
+    """``(offsets [N+1] int32, T)`` of the rows ``padded[n, :lengths[n]]`` packed
+    back to back; the checks and the synchronisation are those :func:`pack_padded`
+    describes."""
     if padded.device.type != "cuda":
         raise RuntimeError(f"padded must be a CUDA tensor (maxsim_b200 has no CPU path); got device {padded.device}")
     N, L_max = padded.shape[0], padded.shape[1]
@@ -106,6 +93,30 @@ def pack_padded(padded: torch.Tensor, lengths: torch.Tensor, *,
             total = int(total_tokens)
     if total_tokens is not None and int(total_tokens) != total:
         raise ValueError(f"total_tokens={int(total_tokens)} does not match lengths.sum()={total}")
+    return offsets, total
+
+
+@_eager
+def pack_padded(padded: torch.Tensor, lengths: torch.Tensor, *,
+                total_tokens: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Pack ``padded [N, L_max, D]`` (CUDA, any dtype) by prefix ``lengths [N]``.
+
+    Returns ``(packed [T, D], offsets [N+1] int32)`` ready for
+    ``score_contrastive*`` (documents) or ``score_pairs_packed*``.
+
+    ``lengths`` may live on the host or on the device.  On the host the offsets
+    are built there and nothing synchronises.  On the device a scan kernel
+    builds them; ``T`` is then read back (one synchronisation) unless the
+    caller passes ``total_tokens``, in which case nothing synchronises and the
+    value is trusted to equal ``lengths.sum()`` (rows beyond it are dropped,
+    never written out of bounds).
+
+    Raises ``ValueError`` for a shape mismatch or, when the lengths are visible
+    to the host, a length outside ``(0, L_max]``.
+    """
+    if padded.dim() < 2:
+        raise ValueError(f"padded must be at least 2-D [N, L_max, ...]; got shape {tuple(padded.shape)}")
+    offsets, total = packed_offsets(padded, lengths, total_tokens)
     return _PackFn.apply(padded, offsets, total), offsets
 
 
@@ -138,6 +149,76 @@ def rerank_order(scores: torch.Tensor) -> torch.Tensor:
     """Full ranking: what ``scores.argsort(dim=1, descending=True)`` gives,
     with ties by ascending index."""
     return rerank_topk(scores, scores.shape[1])[1]
+
+
+def _per_row(name: str, value, rows: int, dtype, device, least: float, most: float):
+    """A sampling parameter: a number in ``(least, most]``, or a ``[rows]`` tensor
+    whose values the kernel looks at."""
+    if isinstance(value, torch.Tensor):
+        if tuple(value.shape) != (rows,):
+            raise ValueError(f"{name} must be a number or have shape [B={rows}]; got shape {tuple(value.shape)}")
+        if value.device != device:
+            raise RuntimeError(f"{name} must be on the scores' device {device}; got {value.device}")
+        if value.is_floating_point() != (dtype == torch.float32) or value.dtype == torch.bool:
+            raise TypeError(f"{name} must hold {'floats' if dtype == torch.float32 else 'integers'}; got {value.dtype}")
+        return value.detach().to(dtype).contiguous()
+    if not least < value <= most:
+        raise ValueError(f"{name} must be in ({least}, {most}]; got {value}")
+    return value
+
+
+@_eager
+def sample_candidates(scores: torch.Tensor, uniforms: torch.Tensor, n: int, *, temperature=1.0,
+                      top_k=None, top_p=None, min_p=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Draw ``n`` different candidates from every row of ``scores [B, C]``, each in
+    proportion to ``exp(score / temperature)`` among those not drawn yet.
+
+    ``uniforms [B, C]`` fp32 are the random numbers, one per candidate, uniform
+    in ``[0, 1)`` (``torch.rand_like``): the same ones give the same draws.
+    Returns ``(indices [B, n] int64, probabilities [B, n] fp32)`` in the order
+    drawn; ``probabilities`` is the candidate's share of the weight the filters
+    keep.  Where a row has fewer candidates left the index is -1 and the
+    probability 0.
+
+    A score that is NaN or ``-inf`` (a masked positive) is no candidate, nor is
+    one more than ``700 * temperature`` below the row's best; of ``+inf`` scores
+    each weighs the same and everything else nothing.  The filters apply in this order, to the
+    candidates best first (equal scores by ascending index):
+
+    * ``top_k`` keeps that many;
+    * ``top_p`` keeps, of those, the ones before which less than ``top_p`` of
+      their weight lies (always the best one);
+    * ``min_p`` keeps the ones that weigh at least ``min_p`` times the best.
+
+    Each parameter is a number or a ``[B]`` tensor on the scores' device, one
+    value per row, which is not checked: a row whose temperature is not
+    positive draws nothing, and ``top_k <= 0``, ``top_p`` outside ``(0, 1)`` or
+    ``min_p`` outside ``(0, 1]`` switch that row's filter off.  ``C`` may be at
+    most 2^20 and ``n`` at most 1024."""
+    if scores.dim() != 2:
+        raise ValueError(f"scores must be 2-D [B, C]; got shape {tuple(scores.shape)}")
+    _v.require_float("scores", scores)
+    if uniforms.shape != scores.shape:
+        raise ValueError(f"uniforms must have the scores' shape {tuple(scores.shape)}; got {tuple(uniforms.shape)}")
+    if uniforms.dtype != torch.float32:
+        raise TypeError(f"uniforms must be float32; got {uniforms.dtype}")
+    B, C = scores.shape
+    if not 0 <= index(n) <= min(C, 1024):
+        raise ValueError(f"n must be in [0, min(C={C}, 1024)]; got {n}")
+    if C > 2 ** 20:
+        raise ValueError(f"scores may have at most 2^20 candidates per row; got {C}")
+    if top_k is None:
+        top_k = 0
+    else:
+        top_k = _per_row("top_k", top_k, B, torch.int32, scores.device, 0, float("inf"))
+        top_k = top_k if isinstance(top_k, torch.Tensor) else min(index(top_k), C)
+    params = [_per_row("temperature", temperature, B, torch.float32, scores.device, 0, float("inf")), top_k,
+              1.0 if top_p is None else _per_row("top_p", top_p, B, torch.float32, scores.device, 0, 1),
+              0.0 if min_p is None or (not isinstance(min_p, torch.Tensor) and min_p == 0)
+              else _per_row("min_p", min_p, B, torch.float32, scores.device, 0, 1)]
+    s = scores.detach().to(torch.float32)
+    s, u = (t if t.stride(1) == 1 or C == 1 else t.contiguous() for t in (s, uniforms.detach()))
+    return _ops.sample_rows(s, u, int(n), *params)
 
 
 _STAGING = {}

@@ -338,3 +338,84 @@ def rank_rows(scores, k):
         idx[b] = order[:k]
     vals = np.take_along_axis(scores, idx, axis=1) if k else np.empty((B, 0), np.float32)
     return vals, idx
+
+
+# ---------------------------------------------------------------------------
+# Row normalisation and sampling (no counterpart in the reference)
+# ---------------------------------------------------------------------------
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension, in 64 bits."""
+    x = np.asarray(x, dtype=np.float64)
+    d = x - x.mean(axis=-1, keepdims=True)
+    h = d / np.sqrt((d * d).mean(axis=-1, keepdims=True) + eps)
+    y = h if weight is None else h * np.asarray(weight, np.float64)
+    return y if bias is None else y + np.asarray(bias, np.float64)
+
+
+def layer_norm_backward(g, x, weight=None, eps=1e-5):
+    """``(grad_x, grad_weight, grad_bias)`` of :func:`layer_norm`; the latter two
+    summed over all leading dimensions."""
+    g, x = np.asarray(g, np.float64), np.asarray(x, np.float64)
+    d = x - x.mean(axis=-1, keepdims=True)
+    r = 1.0 / np.sqrt((d * d).mean(axis=-1, keepdims=True) + eps)
+    h = d * r
+    u = g if weight is None else g * np.asarray(weight, np.float64)
+    dx = r * (u - u.mean(axis=-1, keepdims=True) - h * (u * h).mean(axis=-1, keepdims=True))
+    lead = tuple(range(x.ndim - 1))
+    return dx, (g * h).sum(axis=lead), g.sum(axis=lead)
+
+
+def unit_norm(x, eps=1e-12):
+    """``x / max(|x|, eps)`` over the last dimension, in 64 bits."""
+    x = np.asarray(x, dtype=np.float64)
+    return x / np.maximum(np.sqrt((x * x).sum(axis=-1, keepdims=True)), eps)
+
+
+def unit_norm_backward(g, x, eps=1e-12):
+    g, x = np.asarray(g, np.float64), np.asarray(x, np.float64)
+    n = np.sqrt((x * x).sum(axis=-1, keepdims=True))
+    y = x / np.maximum(n, eps)
+    along = np.where(n > eps, (y * g).sum(axis=-1, keepdims=True), 0.0)
+    return (g - y * along) / np.maximum(n, eps)
+
+
+def sample_candidates(scores, uniforms, n, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """``n`` candidates per row of ``scores [B, C]`` by the exponential race over
+    the given uniforms, from the definition: candidates best first (equal ones by
+    index), cut by top-k, top-p and min-p, and the earliest arrivals of clocks
+    with rates ``exp((s - max) / T)``.  The parameters are numbers or one per row.
+    Returns ``(indices, probabilities)``, -1 and 0 where a row has none left."""
+    scores = np.asarray(scores, dtype=np.float64)
+    uniforms = np.asarray(uniforms, dtype=np.float64)
+    B, C = scores.shape
+    indices = np.full((B, n), -1, dtype=np.int64)
+    shares = np.zeros((B, n))
+    for b in range(B):
+        T, k, p, least = (float(np.broadcast_to(v, (B,))[b]) for v in (temperature, top_k, top_p, min_p))
+        if not T > 0:
+            continue
+        ids = [i for i in range(C) if scores[b, i] > -np.inf]
+        if not ids:
+            continue
+        best = max(scores[b, i] for i in ids)
+        a = {i: 0.0 if scores[b, i] == best else (scores[b, i] - best) / T for i in ids}
+        ids = sorted((i for i in ids if a[i] >= -700.0), key=lambda i: (-scores[b, i], i))
+        if k > 0:
+            ids = ids[: int(k)]
+        if 0 < p < 1:
+            w = np.exp([a[i] for i in ids])
+            limit, before, size = p * w.sum(), 0.0, 0
+            while size < len(ids) and (size == 0 or before < limit):
+                before += w[size]
+                size += 1
+            ids = ids[:size]
+        if 0 < least <= 1:
+            ids = [i for i in ids if np.exp(a[i]) >= least]
+        total = np.exp([a[i] for i in ids]).sum()
+        with np.errstate(divide="ignore", invalid="ignore"):
+            race = {i: a[i] - np.log(-np.log(uniforms[b, i])) for i in ids}
+        drawn = sorted((i for i in ids if not np.isnan(race[i])), key=lambda i: (-race[i], i))[:n]
+        indices[b, : len(drawn)] = drawn
+        shares[b, : len(drawn)] = [np.exp(a[i]) / total for i in drawn]
+    return indices, shares

@@ -1,0 +1,479 @@
+"""Layer norm and unit rows on the GPU, plain and packed, forward and backward,
+against the 64-bit oracle.
+
+Tolerances.  u = 2^-24 is half a step of fp32, u_T that of the rows' type.  A
+sum of D terms taken in any order is off by at most (D - 1) u times the sum of
+their magnitudes; the kernels and anything else that is right take it in chains
+far shorter than D, so K = D / 8 + 16 steps is what these tests grant a sum.
+Every result is rounded once to its type: u_T of its size.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import maxsim_b200 as maxsim
+from maxsim_b200 import _ops
+from oracle import maxsim_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+UT = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TINY = {torch.float32: 2.0 ** -126, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126}  # half a subnormal step, or flushed
+
+
+def f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def steps(dim):
+    return dim / 8 + 16
+
+
+def close(got, want, dtype, slack, what):
+    """|got - want| <= u_T |want| (1 + small) + slack; not finite where want is not."""
+    got = f64(got)
+    assert got.shape == want.shape, what
+    fin = np.isfinite(want)
+    assert np.array_equal(np.isfinite(got), fin), what
+    err = np.abs(got - want)[fin]
+    bound = (1.01 * UT[dtype] * np.abs(want) + slack + TINY[dtype])[fin]
+    bad = err > bound
+    assert not bad.any(), (what, int(bad.sum()), float((err - bound).max()), float(err.max()))
+
+
+def layer_slack(x, w, eps=1e-5):
+    """What fp32 arithmetic may add to a layer norm's rows: the mean is off by
+    K u mean|x|, the variance and the products by K u of themselves."""
+    d = x - x.mean(-1, keepdims=True)
+    r = 1 / np.sqrt((d * d).mean(-1, keepdims=True) + eps)
+    k = steps(x.shape[-1]) * U
+    size = r * np.abs(x).mean(-1, keepdims=True) + np.abs(d * r) + 1
+    return k * size * (1 if w is None else np.abs(w)), k * size
+
+
+def check_layer(x, w, b, g, y, grads, eps=1e-5):
+    """``x``, ``g`` the rows that count as tensors, ``grads`` (dx, dw, db) or None."""
+    dt = x.dtype
+    X, W, B = f64(x), None if w is None else f64(w), None if b is None else f64(b)
+    slack, h_off = layer_slack(X, W, eps)
+    close(y, oracle.layer_norm(X, W, B, eps), dt, slack + (0 if B is None else 4 * U * np.abs(B)), "rows")
+    if grads is None:
+        return
+    G = f64(g)
+    want, dw, db = oracle.layer_norm_backward(G, X, W, eps)
+    u = G if W is None else G * W
+    d = X - X.mean(-1, keepdims=True)
+    r = 1 / np.sqrt((d * d).mean(-1, keepdims=True) + eps)
+    h = np.abs(d * r)
+    mean = lambda v: v.mean(-1, keepdims=True)  # noqa: E731
+    k = steps(X.shape[-1]) * U
+    # the two means by K u of their terms, h by h_off wherever it enters, the factor r by K u
+    slack = r * (2 * k * (np.abs(u) + mean(np.abs(u)) + h * mean(np.abs(u) * h))
+                 + h_off * mean(np.abs(u) * h) + h * mean(np.abs(u) * h_off))
+    if grads[0] is not None:
+        close(grads[0], want, dt, slack, "grad_tokens")
+    rows = X.reshape(-1, X.shape[-1]).shape[0]
+    sums = (rows / 8 + 64) * U
+    flat = lambda v: np.broadcast_to(v, X.shape).reshape(-1, X.shape[-1])  # noqa: E731
+    if grads[1] is not None:
+        close(grads[1], dw, grads[1].dtype, (sums * np.abs(flat(G * h)) + np.abs(flat(G)) * flat(h_off)).sum(0), "grad_weight")
+    if grads[2] is not None:
+        close(grads[2], db, grads[2].dtype, sums * np.abs(flat(G)).sum(0), "grad_bias")
+
+
+def check_unit(x, g, y, dx, eps=1e-12):
+    dt, X = x.dtype, f64(x)
+    k = steps(X.shape[-1]) * U
+    want = oracle.unit_norm(X, eps)
+    close(y, want, dt, k * np.abs(want), "rows")
+    if dx is None:
+        return
+    G = f64(g)
+    m = np.maximum(np.sqrt((X * X).sum(-1, keepdims=True)), eps)
+    slack = 2 * k / m * (np.abs(G) + np.abs(want) * np.abs(want * G).sum(-1, keepdims=True))
+    close(dx, oracle.unit_norm_backward(G, X, eps), dt, slack, "grad_tokens")
+
+
+def rows_of(shape, dtype, seed, scale=1.0, shift=0.5):
+    gen = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=gen) * scale + shift).to(dtype).to(DEV)
+
+
+# widths: one element, below / at / above every tile, odd ones, wide rows
+WIDTHS = [1, 2, 7, 8, 31, 32, 40, 64, 96, 128, 129, 250, 256, 333, 512, 768, 1000, 1024, 1025, 1032, 1536, 2048, 4096,
+          5000, 8192, 8200, 12345]
+MIXES = [(torch.float32, torch.float32), (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16),
+         (torch.float16, torch.float32), (torch.bfloat16, torch.float32)]
+
+
+@pytest.mark.parametrize("dim", WIDTHS)
+@pytest.mark.parametrize("dtype,wtype", MIXES)
+def test_layer_norm_and_gradients(dim, dtype, wtype):
+    rows = 37 if dim < 4096 else 5
+    x = rows_of((rows, dim), dtype, dim).requires_grad_(True)
+    w = rows_of((dim,), wtype, dim + 1, 0.3, 1.0).requires_grad_(True)
+    b = rows_of((dim,), wtype, dim + 2, 0.3, 0.0).requires_grad_(True)
+    g = rows_of((rows, dim), dtype, dim + 3, 1.0, 0.1)
+    y = maxsim.layer_norm(x, w, b)
+    assert y.dtype == dtype and y.shape == x.shape
+    grads = torch.autograd.grad(y, (x, w, b), g)
+    assert [t.dtype for t in grads] == [dtype, wtype, wtype]
+    check_layer(x, w, b, g, y, grads)
+
+
+@pytest.mark.parametrize("dim", WIDTHS)
+@pytest.mark.parametrize("dtype", list(UT))
+def test_unit_norm_and_gradient(dim, dtype):
+    rows = 41 if dim < 4096 else 5
+    x = rows_of((rows, dim), dtype, dim).requires_grad_(True)
+    g = rows_of((rows, dim), dtype, dim + 3, 1.0, 0.1)
+    y = maxsim.unit_norm(x)
+    (dx,) = torch.autograd.grad(y, x, g)
+    check_unit(x, g, y, dx)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 31, 1000, 4097, 70001])
+def test_row_counts(rows):
+    x = rows_of((rows, 72), torch.bfloat16, rows).requires_grad_(True)
+    w = rows_of((72,), torch.float32, 1, 0.3, 1.0).requires_grad_(True)
+    b = rows_of((72,), torch.float32, 2).requires_grad_(True)
+    g = rows_of((rows, 72), torch.bfloat16, 3)
+    y = maxsim.layer_norm(x, w, b)
+    check_layer(x, w, b, g, y, torch.autograd.grad(y, (x, w, b), g))
+    y = maxsim.unit_norm(x)
+    check_unit(x, g, y, torch.autograd.grad(y, x, g)[0])
+
+
+@pytest.mark.parametrize("dim,dtype,wtype", [(768, torch.bfloat16, torch.float32), (128, torch.float16, torch.float16),
+                                             (33, torch.float32, torch.float32), (1500, torch.bfloat16, torch.bfloat16),
+                                             (96, torch.bfloat16, torch.bfloat16), (9000, torch.float16, torch.float32)])
+@pytest.mark.parametrize("where", ["host", "device", "device_total"])
+def test_packed_forms(dim, dtype, wtype, where):
+    N, L = 23, 29
+    lengths = torch.randint(1, L + 1, (N,), generator=torch.Generator().manual_seed(dim), dtype=torch.int32)
+    lengths[0], lengths[1] = L, 1
+    x = rows_of((N, L, dim), dtype, dim)
+    valid = torch.arange(L)[None, :] < lengths[:, None]
+    x[~valid.to(DEV)] = float("nan")  # padding is never read
+    x.requires_grad_(True)
+    w = rows_of((dim,), wtype, 1, 0.3, 1.0).requires_grad_(True)
+    b = rows_of((dim,), wtype, 2).requires_grad_(True)
+    T = int(lengths.sum())
+    g = rows_of((T, dim), dtype, 3)
+    ln = lengths if where == "host" else lengths.to(DEV)
+    kw = {"total_tokens": T} if where == "device_total" else {}
+    kept = x.detach()[valid.to(DEV)]
+    want_offsets = np.concatenate([[0], np.cumsum(lengths.numpy())])
+
+    y, off = maxsim.pack_layer_norm(x, ln, w, b, **kw)
+    assert off.dtype == torch.int32 and off.cpu().tolist() == want_offsets.tolist()
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    assert dx.shape == x.shape and not dx[~valid.to(DEV)].any()
+    check_layer(kept, w, b, g, y, (dx[valid.to(DEV)], dw, db))
+
+    y, off = maxsim.pack_unit_norm(x, ln, **kw)
+    assert off.cpu().tolist() == want_offsets.tolist()
+    (dx,) = torch.autograd.grad(y, x, g)
+    assert not dx[~valid.to(DEV)].any()
+    check_unit(kept, g, y, dx[valid.to(DEV)])
+
+
+def test_packed_form_equals_pack_then_norm_bit_for_bit():
+    x = rows_of((17, 40, 256), torch.bfloat16, 5)
+    lengths = torch.randint(1, 41, (17,), generator=torch.Generator().manual_seed(1))
+    w = rows_of((256,), torch.float32, 1)
+    packed, off = maxsim.pack_padded(x, lengths)
+    y, off2 = maxsim.pack_layer_norm(x, lengths, w)
+    assert torch.equal(off, off2) and torch.equal(y, maxsim.layer_norm(packed, w))
+    y, _ = maxsim.pack_unit_norm(x, lengths)
+    assert torch.equal(y, maxsim.unit_norm(packed))
+
+
+@pytest.mark.parametrize("dim", [64, 100, 768, 1100])
+def test_strided_and_unaligned_rows(dim):
+    """Slices of a larger batch: skipped leading tokens, a narrower last
+    dimension at an odd offset, transposed leading dimensions, expanded rows."""
+    base = rows_of((6, 12, dim + 24), torch.bfloat16, dim)
+    w = rows_of((dim,), torch.bfloat16, 1)
+    g = torch.Generator().manual_seed(0)
+    lengths = torch.randint(1, 11, (6,), generator=g)
+    for view in (base[:, 2:, 8:8 + dim], base[:, 2:, 3:3 + dim], base[1:, :10, 24:], base[..., :dim].transpose(0, 1)[:6, :],
+                 base[:1, :10, :dim].expand(6, 10, dim), base[:, 1:11, :2 * (dim // 2):2]):
+        wv = w[: view.shape[-1]]
+        x = view.detach().requires_grad_(True)
+        gy = rows_of(view.shape, torch.bfloat16, 2)
+        y = maxsim.layer_norm(x, wv)
+        dx, = torch.autograd.grad(y, x, gy)
+        check_layer(view, wv, None, gy, y, (dx, None, None))
+        assert torch.equal(y, maxsim.layer_norm(view.contiguous(), wv))
+        ln = lengths[: view.shape[0]].clamp(max=view.shape[1])
+        p, _ = maxsim.pack_unit_norm(view, ln)
+        assert torch.equal(p, maxsim.pack_unit_norm(view.contiguous(), ln)[0])
+    unaligned = rows_of((37 * dim + 1,), torch.bfloat16, 7)[1:].view(37, dim)
+    check_layer(unaligned, w, None, None, maxsim.layer_norm(unaligned, w), None)
+    w_off = rows_of((dim + 1,), torch.bfloat16, 8)[1:]
+    check_layer(unaligned, w_off, w_off, None, maxsim.layer_norm(unaligned, w_off, w_off), None)
+    many = rows_of((2, 3, 4, dim), torch.float32, 9)
+    assert torch.equal(maxsim.unit_norm(many).view(24, dim), maxsim.unit_norm(many.view(24, dim)))
+    one = rows_of((dim,), torch.float32, 10)
+    assert torch.equal(maxsim.unit_norm(one), maxsim.unit_norm(one[None])[0])
+    # gradients that arrive expanded (from a sum) or transposed
+    x = rows_of((8, dim), torch.float32, 11).requires_grad_(True)
+    (dx,) = torch.autograd.grad(maxsim.unit_norm(x).sum(), x)
+    check_unit(x, torch.ones(8, dim), maxsim.unit_norm(x), dx)
+
+
+def test_parts_of_the_gradient():
+    x = rows_of((50, 200), torch.float16, 0)
+    w = rows_of((200,), torch.float32, 1)
+    b = rows_of((200,), torch.float32, 2)
+    g = rows_of((50, 200), torch.float16, 3)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    full = torch.autograd.grad(maxsim.layer_norm(*leaves), leaves, g)
+    for only in range(3):
+        args = [t.clone().requires_grad_(i == only) for i, t in enumerate((x, w, b))]
+        (got,) = torch.autograd.grad(maxsim.layer_norm(*args), args[only], g)
+        assert torch.equal(got, full[only])
+    # no bias, no weight, nothing to differentiate
+    xa, wa = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    y = maxsim.layer_norm(xa, wa)
+    check_layer(x, w, None, g, y, (*torch.autograd.grad(y, (xa, wa), g), None))
+    y = maxsim.layer_norm(xa)
+    check_layer(x, None, None, g, y, (torch.autograd.grad(y, xa, g)[0], None, None))
+    assert not maxsim.layer_norm(x, w, b).requires_grad
+    # the same tensor as weight and bias: its gradient is the sum of both
+    y = maxsim.layer_norm(x, wa, wa)
+    (dw,) = torch.autograd.grad(y, wa, g)
+    torch.testing.assert_close(dw, full[1] + full[2], rtol=1e-6, atol=1e-6)
+    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad|twice"):
+        first = torch.autograd.grad(maxsim.unit_norm(xa).sum(), xa, create_graph=True)[0]
+        torch.autograd.grad(first.sum(), xa)
+
+
+def test_gradient_against_differences():
+    """Central differences of the kernel's own forward along a direction, summed in
+    64 bits.  fp32 rows are off by about K u each; over sqrt(n) of them that is
+    2e-5 / step, and the truncation of a step of 2^-6 is its square."""
+    gen = torch.Generator().manual_seed(4)
+    x, v, g = (torch.randn(64, 96, generator=gen).to(DEV) for _ in range(3))
+    w, vw, b, vb = (torch.randn(96, generator=gen).to(DEV) for _ in range(4))
+    h = 2.0 ** -6
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y = maxsim.layer_norm(*leaves)
+    dx, dw, db = torch.autograd.grad(y, leaves, g)
+    along = float((dx.double() * v).sum() + (dw.double() * vw).sum() + (db.double() * vb).sum())
+    at = lambda s: float((maxsim.layer_norm(x + s * v, w + s * vw, b + s * vb).double() * g).sum())  # noqa: E731
+    size = float(g.double().norm() * y.double().norm())
+    assert abs((at(h) - at(-h)) / (2 * h) - along) <= size * (h * h + 2e-5 / h)
+    xa = x.clone().requires_grad_(True)
+    (dx,) = torch.autograd.grad(maxsim.unit_norm(xa), xa, g)
+    along = float((dx.double() * v).sum())
+    at = lambda s: float((maxsim.unit_norm(x + s * v).double() * g).sum())  # noqa: E731
+    size = float(g.double().norm() * 8)
+    assert abs((at(h) - at(-h)) / (2 * h) - along) <= size * (h * h + 2e-5 / h)
+
+
+@pytest.mark.parametrize("dtype", list(UT))
+@pytest.mark.parametrize("dim", [24, 33, 768, 1300, 9000])
+def test_extreme_rows(dim, dtype):
+    """Zero rows, constant rows, rows at both ends of the type's range, and rows
+    with an infinity or a NaN; a bad row changes no other."""
+    lim = torch.finfo(dtype)
+    x = rows_of((9, dim), dtype, dim, 1.0, 0.0)
+    x[1] = 0
+    x[2] = 3.0
+    x[3] *= lim.max / 8
+    x[4] *= lim.tiny * 4
+    x[5, dim // 2] = float("inf")
+    x[6, dim // 3] = float("nan")
+    x[7] = lim.max
+    g = rows_of((9, dim), dtype, 1, 1.0, 0.0)
+    xa = x.clone().requires_grad_(True)
+    with np.errstate(all="ignore"):
+        y = maxsim.unit_norm(xa)
+        (dx,) = torch.autograd.grad(y, xa, g)
+        fine = [0, 1, 2, 3, 4, 7, 8]
+        check_unit(x[fine], g[fine], y[fine], None)
+        in_range = [0, 2, 8] if dtype != torch.float16 else [0, 2, 3, 7, 8]
+        check_unit(x[in_range], g[in_range], y[in_range], dx[in_range])
+        assert torch.isfinite(y[fine]).all() and y[1].eq(0).all()
+        # |x| = inf: the infinite entry is inf / inf, the others 0
+        assert torch.isnan(y[5, dim // 2]) and y[5].nan_to_num(0).eq(0).all()
+        assert torch.isnan(y[6]).all()
+        w = rows_of((dim,), torch.float32, 2)
+        y = maxsim.layer_norm(x, w, w)
+        check_layer(x[[0, 1, 2, 8]], w, w, None, y[[0, 1, 2, 8]], None)
+        torch.testing.assert_close(y[1], w.to(dtype))  # a zero row: the bias
+        assert torch.isnan(y[5]).all() and torch.isnan(y[6]).all()
+
+
+def test_small_rows_are_scaled_by_eps():
+    x = rows_of((5, 48), torch.float32, 0) * 1e-4
+    g = rows_of((5, 48), torch.float32, 1)
+    xa = x.clone().requires_grad_(True)
+    y = maxsim.unit_norm(xa, eps=0.5)
+    (dx,) = torch.autograd.grad(y, xa, g)
+    check_unit(x, g, y, dx, eps=0.5)
+    torch.testing.assert_close(dx, g * 2)
+    y = maxsim.layer_norm(x, eps=1e-3)
+    check_layer(x, None, None, None, y, None, eps=1e-3)
+
+
+def test_large_offset_rows_keep_their_variance():
+    """A mean a thousand times the spread: the variance is taken from the deviations."""
+    x = rows_of((20, 640), torch.float32, 0, 1.0, 1000.0)
+    check_layer(x, None, None, None, maxsim.layer_norm(x), None)
+
+
+def test_empty_batches():
+    for shape in ((0, 16), (3, 0, 16), (0, 4, 16)):
+        x = torch.empty(shape, device=DEV, requires_grad=True)
+        w = torch.ones(16, device=DEV, requires_grad=True)
+        y = maxsim.layer_norm(x, w, w)
+        assert y.shape == x.shape
+        dx, dw = torch.autograd.grad(y, (x, w), torch.empty_like(y))
+        assert dx.shape == x.shape and not dw.any()
+        assert maxsim.unit_norm(x).shape == x.shape
+    x = torch.empty(0, 4, 16, device=DEV)
+    y, off = maxsim.pack_layer_norm(x, torch.empty(0, dtype=torch.int32))
+    assert y.shape == (0, 16) and off.tolist() == [0]
+
+
+def test_packed_refusals():
+    x = torch.zeros(4, 8, 16, device=DEV)
+    with pytest.raises(ValueError, match="lengths must be in"):
+        maxsim.pack_layer_norm(x, torch.tensor([1, 2, 9, 3]))
+    with pytest.raises(ValueError, match="lengths must have shape"):
+        maxsim.pack_layer_norm(x, torch.tensor([1, 2, 3]))
+    with pytest.raises(TypeError, match="int32 or int64"):
+        maxsim.pack_unit_norm(x, torch.ones(4))
+    with pytest.raises(ValueError, match="total_tokens"):
+        maxsim.pack_unit_norm(x, torch.tensor([1, 2, 3, 3]), total_tokens=8)
+    with pytest.raises(RuntimeError, match="same device"):
+        maxsim.layer_norm(x, torch.ones(16))
+
+
+def test_a_short_total_drops_rows_and_writes_no_others():
+    """A device total smaller than the lengths' sum: the rows behind it are
+    dropped (as pack_padded does), their gradient is zero, nothing else is written."""
+    x = rows_of((3, 4, 32), torch.float32, 0).requires_grad_(True)
+    w = rows_of((32,), torch.float32, 1).requires_grad_(True)
+    y, off = maxsim.pack_layer_norm(x, torch.tensor([4, 3, 4], device=DEV), w, total_tokens=9)
+    assert y.shape == (9, 32) and off.tolist() == [0, 4, 7, 11]
+    g = rows_of((9, 32), torch.float32, 2)
+    dx, dw = torch.autograd.grad(y, (x, w), g)
+    kept = torch.cat([x.detach()[0], x.detach()[1, :3], x.detach()[2, :2]])
+    assert not dx[1, 3].any() and not dx[2, 2:].any()
+    check_layer(kept, w, None, g, y, (torch.cat([dx[0], dx[1, :3], dx[2, :2]]), dw, None))
+
+
+@pytest.mark.parametrize("dim,dtype", [(768, torch.bfloat16), (333, torch.float32), (5000, torch.float16)])
+def test_equal_calls_give_equal_bits(dim, dtype):
+    x = rows_of((3000, dim), dtype, 0).requires_grad_(True)
+    w = rows_of((dim,), torch.float32, 1).requires_grad_(True)
+    g = rows_of((3000, dim), dtype, 2)
+    runs = []
+    for _ in range(3):
+        y = maxsim.layer_norm(x, w, w)
+        runs.append((y.detach(), *torch.autograd.grad(y, (x, w), g)))
+    for other in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+def test_two_streams_at_once():
+    """Calls on two streams share nothing: results as on one."""
+    xs = [rows_of((4000, 512), torch.bfloat16, i).requires_grad_(True) for i in range(2)]
+    w = rows_of((512,), torch.float32, 9).requires_grad_(True)
+    g = rows_of((4000, 512), torch.bfloat16, 10)
+
+    def call(x):
+        y = maxsim.layer_norm(x, w, w)
+        return (y.detach(), *torch.autograd.grad(y, (x, w), g))
+
+    want = [call(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (x, st) in enumerate(zip(xs, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(call(x))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[i]))
+
+
+def test_training_pass_replays_from_a_graph():
+    N, L, D = 8, 20, 256
+    x = rows_of((N, L, D), torch.bfloat16, 0).requires_grad_(True)
+    w = rows_of((D,), torch.float32, 1).requires_grad_(True)
+    lengths = torch.full((N,), 10, dtype=torch.int32, device=DEV)
+    g = rows_of((N * 10, D), torch.bfloat16, 2)
+
+    def step():
+        y, off = maxsim.pack_layer_norm(x, lengths, w, w, total_tokens=N * 10)
+        return (y.detach(), off, *torch.autograd.grad(y, (x, w), g))
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graphs = []
+    for _ in range(2):  # two graphs over the same leaves, replayed in turn
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out))
+    with torch.no_grad():
+        x.copy_(rows_of((N, L, D), torch.bfloat16, 3))
+        lengths.copy_(torch.tensor([1, 19, 20, 5, 15, 2, 17, 1], dtype=torch.int32))  # the same total
+    for graph, _ in graphs + graphs:
+        graph.replay()
+    torch.cuda.synchronize()
+    want = step()
+    for _, out in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_the_steps_together():
+    """Encoder rows -> layer norm, packed -> projection -> unit rows -> contrastive
+    loss, and back: the gradients against the same chain in torch's own
+    operators in fp32."""
+    torch.manual_seed(0)
+    N, L, H, D, Lq = 6, 30, 192, 64, 16
+    enc = torch.randn(N, L, H, device=DEV)
+    qe = torch.randn(N, Lq, H, device=DEV)
+    lengths = torch.tensor([30, 4, 17, 1, 22, 9])
+    w = (1 + 0.1 * torch.randn(H, device=DEV))
+    b = 0.1 * torch.randn(H, device=DEV)
+    proj = torch.randn(D, H, device=DEV) / H ** 0.5
+
+    def run(kernels):
+        leaves = [t.clone().requires_grad_(True) for t in (enc, qe, w, b, proj)]
+        e, q, ww, bb, pp = leaves
+        if kernels:
+            rows, off = maxsim.pack_layer_norm(e, lengths, ww, bb)
+            docs = maxsim.unit_norm(rows @ pp.T)
+            queries = maxsim.unit_norm(maxsim.layer_norm(q, ww, bb) @ pp.T)
+            loss = maxsim.contrastive_loss(queries, docs, off, temperature=0.5)
+        else:
+            norm = lambda t: torch.nn.functional.layer_norm(t, (H,), ww, bb)  # noqa: E731
+            unit = lambda t: torch.nn.functional.normalize(t, dim=-1)  # noqa: E731
+            docs, queries = unit(norm(e) @ pp.T), unit(norm(q) @ pp.T)
+            sim = torch.einsum("qid,njd->qnij", queries, docs)
+            mask = torch.arange(L)[None, :] >= lengths[:, None]
+            s = sim.masked_fill(mask.to(DEV)[None, :, None, :], float("-inf")).amax(-1).sum(-1)
+            loss = torch.nn.functional.cross_entropy(s / 0.5, torch.arange(N, device=DEV))
+        return [loss.detach(), *torch.autograd.grad(loss, leaves)]
+
+    for name, a, want in zip(("loss", "encoder", "queries", "weight", "bias", "projection"), run(True), run(False)):
+        # both sides fp32: matrix products of 192 terms, K u of the largest entry
+        torch.testing.assert_close(a, want, rtol=1e-4, atol=2e-5 * float(want.abs().max()) + 1e-7, msg=lambda m: name + m)
+    assert _ops.device_status() == 0

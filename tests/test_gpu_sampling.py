@@ -1,0 +1,230 @@
+"""Drawing candidates on the GPU against the 64-bit oracle: the indices have to
+be equal, the probabilities are one fp32 rounding (and a mass rounded to whole
+numbers, below 1e-9) from the oracle's."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import maxsim_b200 as maxsim
+from maxsim_b200 import _ops
+from oracle import maxsim_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+INF = float("inf")
+
+
+def scores_of(B, C, seed, spread=0.6):
+    g = torch.Generator().manual_seed(seed)
+    return (9.5 + spread * torch.randn(B, C, generator=g)), torch.rand(B, C, generator=g)
+
+
+def as_params(kw):
+    return {k: (v.cpu().numpy() if isinstance(v, torch.Tensor) else v) for k, v in kw.items() if v is not None}
+
+
+def check(s, u, n, **kw):
+    got, share = maxsim.sample_candidates(s.to(DEV), u.to(DEV), n, **{
+        k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in kw.items()})
+    assert got.dtype == torch.int64 and share.dtype == torch.float32 and got.shape == share.shape == (s.shape[0], n)
+    want, wshare = oracle.sample_candidates(s.float().numpy(), u.numpy(), n, **as_params(kw))
+    np.testing.assert_array_equal(got.cpu().numpy(), want)
+    np.testing.assert_allclose(share.cpu().numpy(), wshare, rtol=2.0 ** -23, atol=2.0 ** -126)
+    return got, share
+
+
+FILTERS = [dict(), dict(top_k=1), dict(top_k=7), dict(top_p=0.5), dict(top_p=0.999), dict(min_p=0.2), dict(min_p=1.0),
+           dict(top_k=20, top_p=0.8), dict(top_k=13, top_p=0.9, min_p=0.05), dict(top_p=0.97, min_p=0.001)]
+
+
+@pytest.mark.parametrize("C", [1, 2, 3, 31, 32, 33, 255, 256, 257, 1000, 1024, 1025])
+@pytest.mark.parametrize("kw", FILTERS, ids=str)
+def test_filters(C, kw):
+    s, u = scores_of(5, C, C)
+    check(s, u, min(C, 9), temperature=0.3, **kw)
+
+
+@pytest.mark.parametrize("T", [1e-3, 0.05, 1.0, 30.0, INF])
+def test_temperatures(T):
+    s, u = scores_of(6, 300, 1)
+    check(s, u, 20, temperature=T, top_p=0.9)
+    check(s, u, 300, temperature=T)
+
+
+@pytest.mark.parametrize("B,C,n", [(1, 4096, 64), (3, 20000, 32), (2, 5001, 1024), (1, 70000, 16), (300, 64, 64),
+                                   (2, 12289, 300), (2, 40000, 5)])
+def test_long_rows(B, C, n):
+    s, u = scores_of(B, C, C)
+    check(s, u, n, temperature=0.5)
+    check(s, u, n, temperature=0.5, top_k=C // 3, top_p=0.9)
+    check(s, u, n, temperature=0.2, top_p=0.99, min_p=1e-4)
+
+
+def test_masked_rows():
+    """-inf, NaN, the type's lowest value, +inf, and rows with nothing left."""
+    s, u = scores_of(9, 70, 3)
+    s[0, ::2] = -INF
+    s[1, 5:60] = float("nan")
+    s[2, 10:] = torch.finfo(torch.float32).min
+    s[3] = -INF
+    s[4] = float("nan")
+    s[5, [3, 40, 41]] = INF
+    s[6] = torch.finfo(torch.float32).min  # all of them the best: uniform
+    s[7, :69] = -INF
+    s[8, 7] = torch.finfo(torch.float32).max
+    s[8, 8] = -torch.finfo(torch.float32).max
+    for kw in FILTERS:
+        got, share = check(s, u, 12, temperature=0.7, **kw)
+        assert (got[3] == -1).all() and not share[3].any() and (got[4] == -1).all()
+        assert set(got[5].tolist()) <= {3, 40, 41, -1}
+        assert got[7].tolist() == [69] + [-1] * 11
+    half = s.half()
+    check(half, u, 12, temperature=0.7, top_p=0.9)
+    check(s.bfloat16(), u, 12, temperature=0.7, top_k=9)
+
+
+def test_ties_go_to_the_lowest_index():
+    u = torch.full((3, 40), 0.5)
+    s = torch.zeros(3, 40)
+    s[1, 20:] = 1.0
+    s[2, ::3] = -0.0  # equal to +0
+    for kw in FILTERS:
+        check(s, u, 15, **kw)
+    got, _ = check(s, u, 15, top_k=10)
+    assert got[0].tolist() == list(range(10)) + [-1] * 5
+    assert got[1].tolist() == list(range(20, 30)) + [-1] * 5
+    got, _ = check(s, u, 15, top_p=0.5)  # twenty before which less than half lies
+    assert got[0].tolist() == list(range(15))
+    coarse, v = scores_of(8, 600, 4)
+    check(coarse.round(decimals=1), v, 40, top_k=100, temperature=0.4)
+    check(coarse.round(decimals=1), v, 40, top_p=0.77, temperature=0.4)
+    check(coarse.round(decimals=1), (v * 8).floor() / 8, 40, top_p=0.77, temperature=0.4)
+
+
+def test_uniforms_at_and_outside_their_ends():
+    s, u = scores_of(4, 50, 5)
+    u[0, 10:20] = 0.0      # last of the kept, but drawn
+    u[1, 7], u[1, 30] = 1.0, 1.0  # first
+    u[2, 5:9] = float("nan")      # left out, as are values outside [0, 1]
+    u[2, 9], u[2, 10] = -0.5, 1.5
+    u[3] = 0.0
+    got, _ = check(s, u, 50)
+    assert set(got[0, -10:].tolist()) == set(range(10, 20))
+    assert got[1, 0] == 7 and got[1, 1] == 30
+    assert (got[2] == -1).sum() == 6
+    assert got[3].tolist() == list(range(50))
+    check(s, u, 20, top_k=30, top_p=0.9)
+
+
+def test_one_value_per_row():
+    B = 12
+    s, u = scores_of(B, 200, 6)
+    T = torch.linspace(0.1, 2.0, B)
+    T[3], T[4], T[5] = 0.0, -1.0, float("nan")  # rows that draw nothing
+    k = torch.tensor([0, 1, 2, 3, 4, 5, -7, 50, 199, 200, 201, 2 ** 31 - 1], dtype=torch.int32)
+    p = torch.linspace(0.05, 1.1, B)
+    p[7], p[8] = -0.1, float("nan")
+    m = torch.linspace(-0.1, 1.1, B) ** 3
+    check(s, u, 9, temperature=T)
+    check(s, u, 9, top_k=k)
+    check(s, u, 9, top_k=k.long(), temperature=0.4)
+    check(s, u, 9, top_p=p)
+    check(s, u, 9, min_p=m)
+    got, _ = check(s, u, 9, temperature=T, top_k=k, top_p=p, min_p=m)
+    assert (got[3:6] == -1).all()
+
+
+def test_strided_rows():
+    s, u = scores_of(6, 500, 7)
+    S, U = s.to(DEV), u.to(DEV)
+    want = maxsim.sample_candidates(S[:, 3:300].contiguous(), U[:, 100:397].contiguous(), 8, top_p=0.8)
+    got = maxsim.sample_candidates(S[:, 3:300], U[:, 100:397], 8, top_p=0.8)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got = maxsim.sample_candidates(S[:, 3:300].T.contiguous().T, U[:, 100:397], 8, top_p=0.8)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    one = maxsim.sample_candidates(S[:1].expand(4, 500), U[:1].expand(4, 500), 8)
+    assert torch.equal(one[0][0], one[0][3])
+    unaligned = S.flatten()[1:].view(-1)[: 5 * 499].view(5, 499)
+    check(unaligned.cpu(), u[:5, :499], 8, top_k=40)
+
+
+def test_nothing_to_draw():
+    s, u = scores_of(3, 20, 8)
+    got, share = maxsim.sample_candidates(s.to(DEV), u.to(DEV), 0)
+    assert got.shape == share.shape == (3, 0)
+    got, _ = maxsim.sample_candidates(torch.empty(0, 20, device=DEV), torch.empty(0, 20, device=DEV), 5)
+    assert got.shape == (0, 5)
+    got, _ = maxsim.sample_candidates(torch.empty(4, 0, device=DEV), torch.empty(4, 0, device=DEV), 0)
+    assert got.shape == (4, 0)
+    with pytest.raises(RuntimeError, match="scores' device"):
+        maxsim.sample_candidates(s.to(DEV), u.to(DEV), 2, temperature=torch.ones(3))
+
+
+def test_draws_follow_the_weights():
+    """Counts of the first draw over 40000 rows of the same scores, within five
+    standard deviations of the filtered softmax."""
+    row = torch.tensor([1.0, 0.2, 2.0, -INF, 0.7, 1.5, 1.4, -3.0])
+    B, T = 40000, 0.8
+    u = torch.rand(B, 8, generator=torch.Generator().manual_seed(0)).to(DEV)
+    got, share = maxsim.sample_candidates(row.to(DEV).expand(B, 8), u, 3, temperature=T, top_k=5)
+    p = torch.exp(row / T) * (row >= 0.99)
+    p[4] = torch.exp(row[4] / T)
+    p = (p / p.sum()).double().numpy()
+    counts = torch.bincount(got[:, 0], minlength=8).cpu().numpy()
+    assert np.all(np.abs(counts - B * p) <= 5 * np.sqrt(B * p * (1 - p)))
+    srt = got.sort(dim=1).values
+    assert (srt[:, 1:] != srt[:, :-1]).all()
+    np.testing.assert_allclose(share.cpu().numpy(), p[got.cpu().numpy()], rtol=1e-6)
+
+
+def test_replays_from_a_graph_and_repeats_its_bits():
+    s, u = (t.to(DEV) for t in scores_of(64, 3000, 9))
+    T = torch.full((64,), 0.5, device=DEV)
+    call = lambda: maxsim.sample_candidates(s, u, 16, temperature=T, top_k=500, top_p=0.9)  # noqa: E731
+    first = call()
+    assert all(torch.equal(a, b) for a, b in zip(first, call()))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        call()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    s2, u2 = scores_of(64, 3000, 10)
+    s.copy_(s2)
+    u.copy_(u2)
+    T.fill_(0.3)
+    graph.replay()
+    torch.cuda.synchronize()
+    want = call()
+    assert all(torch.equal(a, b) for a, b in zip(out, want)) and not torch.equal(out[0], first[0])
+
+
+def test_hard_negatives_for_a_training_step():
+    """Scores of a contrastive batch -> negatives drawn with the positive masked ->
+    the candidates gathered -> the padded training operator and its gradients."""
+    torch.manual_seed(0)
+    Nq, Lq, D, L, n = 10, 16, 64, 24, 4
+    q = maxsim.unit_norm(torch.randn(Nq, Lq, D, device=DEV)).half()
+    enc = torch.randn(Nq, L, D, device=DEV)
+    lengths = torch.randint(3, L + 1, (Nq,), dtype=torch.int32)
+    docs, off = maxsim.pack_unit_norm(enc.half(), lengths)
+    scores = maxsim.score_contrastive(q, docs, off)
+    masked = scores.clone().fill_diagonal_(-INF)
+    u = torch.rand(masked.shape, device=DEV)
+    neg, _ = check(masked.cpu(), u.cpu(), n, temperature=0.5, top_k=6)
+    assert (neg >= 0).all() and (neg != torch.arange(Nq, device=DEV)[:, None]).all()
+    chosen = torch.cat([torch.arange(Nq, device=DEV)[:, None], neg], 1)
+    cand = maxsim.unpack_packed(docs, off, L)[chosen].detach().requires_grad_(True)
+    qa = q.clone().requires_grad_(True)
+    s = maxsim.score_candidates_padded_train(qa, cand, torch.full((Nq,), Lq, dtype=torch.int32, device=DEV),
+                                             lengths.to(DEV)[chosen])
+    torch.testing.assert_close(s.detach(), torch.gather(scores, 1, chosen), rtol=2e-2, atol=1e-2)
+    loss = torch.nn.functional.cross_entropy(s / 0.5, torch.zeros(Nq, dtype=torch.long, device=DEV))
+    gq, gd = torch.autograd.grad(loss, (qa, cand))
+    assert torch.isfinite(gq).all() and torch.isfinite(gd).all() and gq.abs().sum() > 0
+    assert _ops.device_status() == 0
