@@ -18,6 +18,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace maxsim {
 namespace norm {
 
@@ -35,32 +37,163 @@ template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float
   return __float2bfloat16_rn(v);
 }
 
-// Which rows there are, where a row is read and which packed row it is.
+// Which rows there are.  Token row j of segment n starts n * segment_stride + j *
+// row_stride elements into the tokens; with offsets it counts for j < offsets[n+1] -
+// offsets[n] and is row offsets[n] + j of the packed tensors, without them every row
+// counts and is row n * L_max + j.
 struct Rows {
-  int64_t segment_stride, row_stride;  // of the token rows, in elements
-  const int32_t* offsets;              // [n_segments + 1], or null: every row counts
-  int64_t packed_rows;                 // rows at or beyond are never touched
-  uint32_t n_slots, L_max;             // n_slots = n_segments * L_max
-  int dim;
+  int64_t segment_stride, row_stride;  // in elements
+  const int32_t* offsets;              // [n_segments + 1], or null
+  int32_t n_segments, L_max;
+  int32_t rows;   // packed rows: the ones at or beyond are never touched
+  int32_t chunk;  // consecutive packed rows of one unit (a warp, or a CTA)
+  int32_t dim;
+
+  __device__ __forceinline__ int32_t start(int32_t n) const { return offsets ? offsets[n] : n * L_max; }
+  // Packed rows that belong to a segment.
+  __device__ __forceinline__ int32_t used() const { return min(rows, start(n_segments)); }
 };
 
-struct Place {
-  int64_t from;  // first element of the token row
-  int64_t to;    // packed row, -1 for padding
+// Walks the packed rows upwards and knows the segment it is in.  A unit looks its first segment up
+// once (32 offsets at a time) and then only steps: no division and, within a
+// segment, no load.  Offsets that are none (decreasing, longer than L_max) lead to a
+// token row of the batch, never out of it.
+struct Walker {
+  int32_t n, first, end;  // segment n is packed rows [first, end)
+
+  __device__ __forceinline__ void find(const Rows& t, int32_t row) {  // all lanes of a warp, same row
+    if (!t.offsets) {
+      n = min(row / t.L_max, t.n_segments - 1);
+    } else {
+      const int lane = threadIdx.x & 31;
+      int32_t lo = 0, size = t.n_segments;
+      while (size > 1) {  // the last segment that starts at or before the row lies in [lo, lo + size)
+        const int32_t step = (size + 31) >> 5;
+        const int32_t at = lane * step;
+        const bool yes = at < size && t.offsets[lo + at] <= row;
+        const int32_t k = max(__popc(__ballot_sync(0xffffffffu, yes)) - 1, 0) * step;
+        lo += k;
+        size = min(step, size - k);
+      }
+      n = lo;
+    }
+    first = t.start(n);
+    end = t.start(n + 1);
+  }
+  __device__ __forceinline__ void seek(const Rows& t, int32_t row) {
+    while (row >= end && n + 1 < t.n_segments) {
+      ++n;
+      first = end;
+      end = t.start(n + 1);
+    }
+  }
+  __device__ __forceinline__ int32_t token(const Rows& t, int32_t row) const {  // in the segment
+    return (int32_t)min((uint32_t)(row - first), (uint32_t)(t.L_max - 1));
+  }
+  __device__ __forceinline__ int64_t from(const Rows& t, int32_t row) const {
+    return n * t.segment_stride + token(t, row) * t.row_stride;
+  }
+  __device__ __forceinline__ int64_t slot(const Rows& t, int32_t row) const {
+    return (int64_t)n * t.L_max + token(t, row);
+  }
 };
 
-__device__ __forceinline__ Place place_of(const Rows& t, uint32_t slot) {
-  const uint32_t n = slot / t.L_max, j = slot - n * t.L_max;
-  Place p;
-  p.from = (int64_t)n * t.segment_stride + (int64_t)j * t.row_stride;
-  p.to = slot;
-  if (t.offsets) {
-    const int64_t o0 = __ldg(t.offsets + n), o1 = __ldg(t.offsets + n + 1);
-    p.to = o0 + j;
-    if (o0 < 0 || p.to >= o1 || p.to >= t.packed_rows) p.to = -1;
+// E consecutive elements of a row, moved as one access (16, 4 or 2 bytes).
+// Plain loads throughout: __ldg of a 16-bit element is an asm statement that the
+// compiler may move in front of the test for a null pointer.
+template <int BYTES> struct Word { using type = uint4; };
+template <> struct Word<8> { using type = uint2; };
+template <> struct Word<4> { using type = uint32_t; };
+template <> struct Word<2> { using type = uint16_t; };
+template <typename T, int E>
+struct alignas(sizeof(T) * E) Pack {
+  T v[E];
+};
+template <typename T, int E>
+__device__ __forceinline__ Pack<T, E> load_pack(const void* p) {
+  using U = typename Word<sizeof(T) * E>::type;
+  Pack<T, E> out;
+  *reinterpret_cast<U*>(&out) = *reinterpret_cast<const U*>(p);
+  return out;
+}
+template <typename T, int E>
+__device__ __forceinline__ void store_pack(void* p, const Pack<T, E>& x) {
+  using U = typename Word<sizeof(T) * E>::type;
+  *reinterpret_cast<U*>(p) = *reinterpret_cast<const U*>(&x);
+}
+
+template <typename T, int E>
+__device__ __forceinline__ void expand(const Pack<T, E>& p, float (&f)[E]) {
+  if constexpr (sizeof(T) == 2 && E % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      const uint32_t u = reinterpret_cast<const uint32_t*>(&p)[i];
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {  // the upper half of a float
+        f[2 * i] = __uint_as_float(u << 16);
+        f[2 * i + 1] = __uint_as_float(u & 0xffff0000u);
+      } else {
+        const float2 both = __half22float2(reinterpret_cast<const __half2&>(u));
+        f[2 * i] = both.x;
+        f[2 * i + 1] = both.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = widen(p.v[e]);
+  }
+}
+template <typename T, int E>
+__device__ __forceinline__ Pack<T, E> compress(const float (&f)[E]) {
+  Pack<T, E> p;
+  if constexpr (sizeof(T) == 2 && E % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        reinterpret_cast<__nv_bfloat162*>(&p)[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      else
+        reinterpret_cast<__half2*>(&p)[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) p.v[e] = narrow<T>(f[e]);
   }
   return p;
 }
+
+// A layer norm's weight or bias: float, or of the rows' type.
+struct Affine {
+  const void* p;  // null: none
+  bool f32;
+  template <typename T>
+  __device__ __forceinline__ float at(int c) const {
+    return f32 ? static_cast<const float*>(p)[c] : widen(static_cast<const T*>(p)[c]);
+  }
+};
+
+// A vector of the row's width in shared memory, as floats.  A thread's pack of
+// eight lies in two halves, so that neighbouring packs of a half meet no bank twice.
+template <int E>
+struct Wide {
+  static constexpr int kPart = E < 4 ? E : 4;
+  float* words;
+  int packs;  // of the row
+  static constexpr __host__ __device__ int bytes(int dim) { return (dim + E - 1) / E * E * 4; }
+  template <typename T>
+  __device__ __forceinline__ void fill(const Affine& a, int dim, float none) const {
+    for (int c = threadIdx.x; c < packs * E; c += blockDim.x) {
+      const int pack = c / E, e = c % E;
+      words[((e / kPart) * packs + pack) * kPart + e % kPart] = a.p && c < dim ? a.at<T>(c) : none;
+    }
+  }
+  __device__ __forceinline__ void get(int pack, float (&w)[E]) const {
+#pragma unroll
+    for (int i = 0; i < E / kPart; ++i) {
+      const Pack<float, kPart> f = load_pack<float, kPart>(words + (i * packs + pack) * kPart);
+#pragma unroll
+      for (int e = 0; e < kPart; ++e) w[i * kPart + e] = f.v[e];
+    }
+  }
+};
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -73,15 +206,18 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// The factors of a unit row: y_i = (x_i * pre) * inv.  A sum of squares near the
-// ends of the 32-bit range is taken again over x / max|x| (pre = 1 / max|x|).
+// The factors of a unit row: y_i = (x_i * pre) * inv.  Nearly every row is plain: its
+// sum of squares is well inside the 32-bit range and above eps^2.  For the others
+// the sum is taken again over x / max|x|.
 struct UnitScale {
   float pre, inv;
   bool clamped;  // |x| <= eps: y = x / eps
 };
-__device__ __forceinline__ bool squares_out_of_range(float ss) { return ss > 1e37f || ss < 1e-30f; }
-__device__ __forceinline__ UnitScale unit_scale(float ss, float top, bool scaled, float eps) {
-  // |x| = top * sqrt(ss) when scaled by top, else sqrt(ss); a NaN stays one
+__device__ __forceinline__ float least_square(float eps) { return fmaxf(1e-30f, 1.0001f * eps * eps); }
+__device__ __forceinline__ bool plain_square(float ss, float least) { return ss > least && ss < 1e37f; }
+// `ss` is that of x / top where top is positive and finite, else of x; a NaN stays one.
+__device__ __forceinline__ UnitScale unit_scale(float ss, float top, float eps) {
+  const bool scaled = top > 0.f && top < INFINITY;
   const float norm = scaled ? top * sqrtf(ss) : sqrtf(ss);
   UnitScale u;
   if (norm == INFINITY && !scaled) {  // an infinity in the row: finite / inf = 0, inf / inf = NaN
@@ -96,19 +232,564 @@ __device__ __forceinline__ UnitScale unit_scale(float ss, float top, bool scaled
   return u;
 }
 
-// One warp per row, three passes over it.
-template <typename T, typename W, int KIND>
+// ---------------------------------------------------------------------------
+// Rows shared by a team of TEAM threads (8, 16 or 32 lanes of a warp, or a CTA of
+// 128); a thread has V packs of E elements of a row.  Every element is read once and
+// written once.
+//
+// HBM-bound: what counts is bytes in flight.  Every thread copies its own packs of the
+// next rows into a ring in shared memory (cp.async) and reads back nothing but
+// what it copied itself, so the ring needs no barrier; the reductions and the store of a row run
+// under the loads of the next kStages - 1.  Packs of 2 bytes (rows of 16-bit elements that do
+// not start on 4 bytes) cannot be copied that way and are loaded in place.
+// ---------------------------------------------------------------------------
+constexpr int kWide = 128;  // threads of a team that is a CTA
+
+template <int TEAM>
+constexpr int kCtaThreads = TEAM > 32 ? TEAM : kThreads;
+
+// Threads an SM is to hold at once: what the registers are cut to.
+template <int E, int V>
+constexpr int kForwardThreads = V * E <= 8 ? 1024 : V * E <= 16 ? 768 : 512;
+template <int KIND, int E, int V>
+constexpr int kBackwardThreads = KIND == kUnit ? kForwardThreads<E, V> : V * E <= 8 ? 768 : 512;
+
+template <typename T, int E>
+constexpr bool kRing = sizeof(T) * E >= 4;
+
+constexpr int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// Rows in the ring (one of them in use): as many as 200 KB of shared memory hold, 2 to 4.
+template <typename T, int E, int TEAM, int V, int TENSORS, int SM_THREADS>
+constexpr int kStages = clamp_int(200 * 1024 / (SM_THREADS * V * E * (int)sizeof(T) * TENSORS), 2, 4);
+template <typename T, int E, int TEAM, int V, int TENSORS, int SM_THREADS>
+constexpr int kRingBytes =
+    kRing<T, E> ? kStages<T, E, TEAM, V, TENSORS, SM_THREADS> * kCtaThreads<TEAM> * V * E * (int)sizeof(T) * TENSORS : 0;
+
+// The column sums at the end of the backward kernel take the ring's place: element e
+// of a pack lies e * kSumPitch on, which meets no bank twice, written or read.
+template <int E, int TEAM>
+constexpr int kSumPitch = TEAM + 32 / E;
+template <int E, int TEAM>
+constexpr int kSumBytes = 2 * (kCtaThreads<TEAM> / TEAM) * E * kSumPitch<E, TEAM> * 4;
+
+// What lies before the weights in the backward kernel's shared memory.
+template <typename T, int KIND, int E, int TEAM, int V>
+constexpr int kBackwardBytes = [] {
+  const int ring = kRingBytes<T, E, TEAM, V, 2, kBackwardThreads<KIND, E, V>>;
+  const int sums = KIND == kLayer ? kSumBytes<E, TEAM> : 0;
+  return ring > sums ? ring : sums;
+}();
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* shared, const void* global) {
+  const uint32_t to = (uint32_t)__cvta_generic_to_shared(shared);
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(global) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(global) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
+// Sums over a team.  Teams of one warp or less use shuffles: all lanes of the
+// warp take part, whether their row counts or not.  A CTA team takes one
+// barrier per sum: the next sum uses the other half of the words.
+template <int TEAM>
+struct Team {
+  float* words;  // [2][2][TEAM / 32] for a CTA
+  int half = 0;
+  __device__ __forceinline__ Team(float* w) : words(w) {}
+
+  template <typename Op>
+  __device__ __forceinline__ float2 reduce(float a, float b, Op op) {
+#pragma unroll
+    for (int off = (TEAM > 32 ? 32 : TEAM) / 2; off > 0; off >>= 1) {
+      a = op(a, __shfl_xor_sync(0xffffffffu, a, off));
+      b = op(b, __shfl_xor_sync(0xffffffffu, b, off));
+    }
+    if constexpr (TEAM > 32) {
+      constexpr int W = TEAM / 32;
+      float* mine = words + half * 2 * W;
+      half ^= 1;
+      if ((threadIdx.x & 31) == 0) {
+        mine[threadIdx.x >> 5] = a;
+        mine[W + (threadIdx.x >> 5)] = b;
+      }
+      __syncthreads();
+      a = mine[0];
+      b = mine[W];
+#pragma unroll
+      for (int w = 1; w < W; ++w) {
+        a = op(a, mine[w]);
+        b = op(b, mine[W + w]);
+      }
+    }
+    return make_float2(a, b);
+  }
+  __device__ __forceinline__ float2 sums(float a, float b) {
+    return reduce(a, b, [](float x, float y) { return x + y; });
+  }
+  // The second value is unused and goes with the optimiser (for a CTA it costs a word).
+  __device__ __forceinline__ float sum(float a) { return sums(a, 0.f).x; }
+  __device__ __forceinline__ float max(float a) {
+    return reduce(a, 0.f, [](float x, float y) { return fmaxf(x, y); }).x;
+  }
+  // Whether any team that has to run the same shuffles says yes.
+  __device__ __forceinline__ bool any(bool v) const {
+    return TEAM > 32 ? v : (bool)__any_sync(0xffffffffu, v);
+  }
+};
+
+// One thread's packs of the rows ahead, of TENSORS tensors.
+template <typename T, int E, int TEAM, int V, int TENSORS, int STAGES>
+struct Ring {
+  static constexpr int kBytes = E * (int)sizeof(T);
+  static constexpr int kCta = kCtaThreads<TEAM>;
+  char* mine;
+  int lane;
+  __device__ __forceinline__ Ring(char* shared) : mine(shared + threadIdx.x * kBytes), lane(threadIdx.x % TEAM) {}
+  __device__ __forceinline__ char* at(int stage, int tensor, int v) const {
+    return mine + ((stage * TENSORS + tensor) * V + v) * (kCta * kBytes);
+  }
+  __device__ __forceinline__ void copy(int stage, int tensor, const T* row, int dim) const {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = (lane + TEAM * v) * E;
+      if (c < dim) copy_async<kBytes>(at(stage, tensor, v), row + c);
+    }
+  }
+  __device__ __forceinline__ Pack<T, E> pack(int stage, int tensor, int v) const {
+    return load_pack<T, E>(at(stage, tensor, v));
+  }
+};
+
+// The packed rows of a team: a unit (a warp, or the CTA of a wide team) takes t.chunk
+// consecutive ones and its teams take them in turn.
+template <int TEAM>
+struct Turn {
+  static constexpr int kRows = TEAM >= 32 ? 1 : 32 / TEAM;  // rows of a unit at a time
+  int32_t begin, end, mine;  // of the unit; the team's place in its turn
+  __device__ __forceinline__ Turn(const Rows& t) {
+    const int64_t unit = TEAM > 32 ? blockIdx.x : (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    const int64_t from = unit * t.chunk, used = t.used();
+    begin = (int32_t)min(from, used);
+    end = (int32_t)min(from + t.chunk, used);
+    mine = TEAM >= 32 ? 0 : (threadIdx.x & 31) / TEAM;
+  }
+};
+
+template <typename T, int KIND, int E, int TEAM, int V>
+__global__ void __launch_bounds__(kCtaThreads<TEAM>, kForwardThreads<E, V> / kCtaThreads<TEAM>)
+forward_rows_kernel(const T* __restrict__ tokens, const __grid_constant__ Rows t, Affine weight, Affine bias,
+                    T* __restrict__ out, float* __restrict__ mean, float* __restrict__ rstd, float eps) {
+  constexpr int S = kRing<T, E> ? kStages<T, E, TEAM, V, 1, kForwardThreads<E, V>> : 1;
+  extern __shared__ __align__(16) char shared[];
+  __shared__ float words[TEAM > 32 ? TEAM / 8 : 1];
+  Team<TEAM> team(words);
+  Ring<T, E, TEAM, V, 1, S> ring(shared);
+  const int lane = threadIdx.x % TEAM;
+  const float per = 1.0f / t.dim, least = least_square(eps);
+  const Turn<TEAM> turn(t);
+  constexpr int R = Turn<TEAM>::kRows;
+
+  Walker ahead;
+  if (turn.begin < turn.end) ahead.find(t, turn.begin);
+  const auto copy = [&](int stage, int32_t row) {
+    if (row < turn.end) {
+      ahead.seek(t, row);
+      ring.copy(stage, 0, tokens + ahead.from(t, row), t.dim);
+    }
+    copies_commit();
+  };
+  if constexpr (kRing<T, E>) {
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) copy(i, turn.begin + turn.mine + i * R);
+  }
+  const int packs = (t.dim + E - 1) / E;
+  float* const after = reinterpret_cast<float*>(shared + kRingBytes<T, E, TEAM, V, 1, kForwardThreads<E, V>>);
+  const Wide<E> w{after, packs}, b{after + packs * E, packs};
+  if constexpr (KIND == kLayer) {
+    w.template fill<T>(weight, t.dim, 1.0f);
+    b.template fill<T>(bias, t.dim, 0.0f);
+    __syncthreads();
+  }
+  int stage = 0;
+  for (int32_t at = turn.begin; at < turn.end; at += R) {
+    const int32_t row = at + turn.mine;
+    const bool there = row < turn.end;
+    if constexpr (kRing<T, E>) {
+      copy(stage == 0 ? S - 1 : stage - 1, row + (S - 1) * R);
+      copies_wait<S - 1>();
+    } else if (there) {
+      ahead.seek(t, row);
+    }
+    float f[V][E];
+    float s = 0.f, ss = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = (lane + TEAM * v) * E;
+      if (there && c < t.dim) {
+        if constexpr (kRing<T, E>) expand(ring.pack(stage, 0, v), f[v]);
+        else expand(load_pack<T, E>(tokens + ahead.from(t, row) + c), f[v]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[v][e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (KIND == kLayer) s += f[v][e];
+        else ss += f[v][e] * f[v][e];
+      }
+    }
+    stage = stage == S - 1 ? 0 : stage + 1;
+    if constexpr (KIND == kLayer) {
+      const float mu = team.sum(s) * per;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const bool in = (lane + TEAM * v) * E < t.dim;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          f[v][e] = in ? f[v][e] - mu : 0.f;
+          ss += f[v][e] * f[v][e];
+        }
+      }
+      const float r = rsqrtf(team.sum(ss) * per + eps);
+      if (there) {
+        T* const y = out + (int64_t)row * t.dim;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int c = (lane + TEAM * v) * E;
+          if (c < t.dim) {
+            float wv[E], bv[E];
+            w.get(lane + TEAM * v, wv);
+            b.get(lane + TEAM * v, bv);
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[v][e] = f[v][e] * r * wv[e] + bv[e];
+            store_pack<T, E>(y + c, compress<T, E>(f[v]));
+          }
+        }
+        if (mean && lane == 0) {
+          mean[row] = mu;
+          rstd[row] = r;
+        }
+      }
+    } else {
+      ss = team.sum(ss);
+      float inv = rsqrtf(ss);
+      const bool plain = plain_square(ss, least) || !there;
+      if (team.any(!plain)) {
+        float top = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+          for (int e = 0; e < E; ++e) top = fmaxf(top, fabsf(f[v][e]));
+        top = team.max(top);
+        const bool scaled = top > 0.f && top < INFINITY;
+        float again = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+          for (int e = 0; e < E; ++e) again += scaled ? (f[v][e] / top) * (f[v][e] / top) : 0.f;
+        again = team.sum(again);
+        if (!plain) {
+          const UnitScale u = unit_scale(scaled ? again : ss, top, eps);
+          inv = u.inv;
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[v][e] *= u.pre;
+        }
+      }
+      if (there) {
+        T* const y = out + (int64_t)row * t.dim;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int c = (lane + TEAM * v) * E;
+          if (c < t.dim) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) f[v][e] *= inv;
+            store_pack<T, E>(y + c, compress<T, E>(f[v]));
+          }
+        }
+      }
+    }
+  }
+}
+
+// Zeroes the token rows that do not count, in grad_tokens: the units share the
+// slots, and what is not valid of a segment lies in one piece.
+template <typename T, int E>
+__device__ __forceinline__ void zero_padding(const Rows& t, T* grad_tokens, int64_t unit, int64_t units, int lane, int team) {
+  const int64_t slots = (int64_t)t.n_segments * t.L_max, share = (slots + units - 1) / units;
+  const int64_t lo = unit * share, hi = min(lo + share, slots);
+  const int32_t used = t.used();
+  Pack<T, E> zero;
+#pragma unroll
+  for (int e = 0; e < E; ++e) zero.v[e] = narrow<T>(0.f);
+  for (int64_t n = lo / t.L_max; n * t.L_max < hi; ++n) {
+    const int32_t first = t.offsets[n];
+    const int32_t len = max(min(min(t.offsets[n + 1], used) - first, t.L_max), 0);
+    const int64_t from = max(lo, n * t.L_max + len) * t.dim, to = min(hi, (n + 1) * t.L_max) * t.dim;
+    for (int64_t c = from + lane * E; c < to; c += team * E) store_pack<T, E>(grad_tokens + c, zero);
+  }
+}
+
+// The gradient of the rows and, for a layer norm, a CTA's share of the weight's
+// and bias's: a thread meets the same columns in every row, so it sums
+// g h and g in registers over all its rows; at the end the teams of the CTA add up
+// through shared memory and the CTA writes one row of partial [2][gridDim.x][dim].
+// The row's packs are read twice from the ring (once for the sums, once for the result):
+// the registers go to the column sums.
+template <typename T, int KIND, int E, int TEAM, int V>
+__global__ void __launch_bounds__(kCtaThreads<TEAM>, kBackwardThreads<KIND, E, V> / kCtaThreads<TEAM>)
+backward_rows_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, const __grid_constant__ Rows t,
+                     Affine weight, const float* __restrict__ mean, const float* __restrict__ rstd,
+                     T* __restrict__ grad_tokens, float* __restrict__ partial, float eps) {
+  constexpr int kCta = kCtaThreads<TEAM>;
+  constexpr int S = kRing<T, E> ? kStages<T, E, TEAM, V, 2, kBackwardThreads<KIND, E, V>> : 1;
+  constexpr int kFixed = kBackwardBytes<T, KIND, E, TEAM, V>;
+  extern __shared__ __align__(16) char shared[];
+  __shared__ float words[TEAM > 32 ? TEAM / 8 : 1];
+  Team<TEAM> team(words);
+  Ring<T, E, TEAM, V, 2, S> ring(shared);
+  const int lane = threadIdx.x % TEAM;
+  const float per = 1.0f / t.dim, least = least_square(eps);
+  float dw[KIND == kLayer ? V : 1][E], db[KIND == kLayer ? V : 1][E];
+  if constexpr (KIND == kLayer) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int e = 0; e < E; ++e) dw[v][e] = db[v][e] = 0.f;
+  }
+  const Turn<TEAM> turn(t);
+  constexpr int R = Turn<TEAM>::kRows;
+  Walker ahead, here;
+  if (turn.begin < turn.end) ahead.find(t, turn.begin);
+  here = ahead;
+  const auto copy = [&](int stage, int32_t row) {
+    if (row < turn.end) {
+      ahead.seek(t, row);
+      ring.copy(stage, 0, tokens + ahead.from(t, row), t.dim);
+      ring.copy(stage, 1, grad + (int64_t)row * t.dim, t.dim);
+    }
+    copies_commit();
+  };
+  if constexpr (kRing<T, E>) {
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) copy(i, turn.begin + turn.mine + i * R);
+  }
+  const int packs = (t.dim + E - 1) / E;
+  const Wide<E> w{reinterpret_cast<float*>(shared + kFixed), packs};
+  if constexpr (KIND == kLayer) {
+    w.template fill<T>(weight, t.dim, 1.0f);
+    __syncthreads();
+  }
+  if (t.offsets && grad_tokens) {
+    if (TEAM > 32) zero_padding<T, E>(t, grad_tokens, blockIdx.x, gridDim.x, threadIdx.x, TEAM);
+    else zero_padding<T, E>(t, grad_tokens, (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5),
+                            (int64_t)gridDim.x * (kThreads / 32), threadIdx.x & 31, 32);
+  }
+  int stage = 0;
+  for (int32_t at = turn.begin; at < turn.end; at += R) {
+    const int32_t row = at + turn.mine;
+    const bool there = row < turn.end;
+    float mu = 0.f, r = 0.f;
+    if (there) {
+      here.seek(t, row);
+      if (KIND == kLayer) {
+        mu = mean[row];
+        r = rstd[row];
+      }
+    }
+    if constexpr (kRing<T, E>) {
+      copy(stage == 0 ? S - 1 : stage - 1, row + (S - 1) * R);
+      copies_wait<S - 1>();
+    }
+    // pack v of the row and of its gradient
+    const auto packs_of = [&](int v, float (&x)[E], float (&g)[E]) {
+      if constexpr (kRing<T, E>) {
+        expand(ring.pack(stage, 0, v), x);
+        expand(ring.pack(stage, 1, v), g);
+      } else {
+        const int c = (lane + TEAM * v) * E;
+        expand(load_pack<T, E>(tokens + here.from(t, row) + c), x);
+        expand(load_pack<T, E>(grad + (int64_t)row * t.dim + c), g);
+      }
+    };
+    T* const dx = grad_tokens + (there ? here.slot(t, row) * t.dim : 0);
+    const bool store = grad_tokens && there;
+    if constexpr (KIND == kLayer) {
+      float su = 0.f, suh = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (there && (lane + TEAM * v) * E < t.dim) {
+          float x[E], g[E], wv[E];
+          packs_of(v, x, g);
+          w.get(lane + TEAM * v, wv);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float h = (x[e] - mu) * r, u = g[e] * wv[e];
+            su += u;
+            suh += u * h;
+            dw[v][e] += g[e] * h;
+            db[v][e] += g[e];
+          }
+        }
+      }
+      const float2 both = team.sums(su, suh);
+      // dx = r (u - mean(u) - h mean(u h))
+      const float minus_u = -r * (both.x * per), minus_h = -r * (both.y * per);
+      asm volatile("" ::: "memory");  // read the packs again instead of keeping them
+      if (store) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int c = (lane + TEAM * v) * E;
+          if (c < t.dim) {
+            float x[E], g[E], wv[E];
+            packs_of(v, x, g);
+            w.get(lane + TEAM * v, wv);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              const float h = (x[e] - mu) * r;
+              x[e] = g[e] * wv[e] * r + (h * minus_h + minus_u);
+            }
+            store_pack<T, E>(dx + c, compress<T, E>(x));
+          }
+        }
+      }
+    } else {
+      float x[V][E], g[V][E];
+      float ss = 0.f, xg = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (there && (lane + TEAM * v) * E < t.dim) {
+          packs_of(v, x[v], g[v]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) x[v][e] = g[v][e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          ss += x[v][e] * x[v][e];
+          xg += x[v][e] * g[v][e];
+        }
+      }
+      const float2 both = team.sums(ss, xg);
+      ss = both.x;
+      xg = both.y;
+      float inv = rsqrtf(ss), pre = 1.0f, along = xg * inv;  // along: y . g
+      const bool plain = plain_square(ss, least) || !there;
+      if (team.any(!plain)) {
+        float top = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+          for (int e = 0; e < E; ++e) top = fmaxf(top, fabsf(x[v][e]));
+        top = team.max(top);
+        const bool scaled = top > 0.f && top < INFINITY;
+        float ss2 = 0.f, xg2 = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float xv = scaled ? x[v][e] / top : 0.f;
+            ss2 += xv * xv;
+            xg2 += xv * g[v][e];
+          }
+        const float2 again = team.sums(ss2, xg2);
+        if (!plain) {
+          const UnitScale u = unit_scale(scaled ? again.x : ss, top, eps);
+          inv = u.inv;
+          pre = u.pre;
+          along = u.clamped ? 0.0f : (scaled ? again.y : xg) * inv;
+        }
+      }
+      if (store) {
+        const float scale = inv * pre, minus = -along * scale;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int c = (lane + TEAM * v) * E;
+          if (c < t.dim) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[v][e] = g[v][e] * scale + x[v][e] * pre * inv * minus;
+            store_pack<T, E>(dx + c, compress<T, E>(x[v]));
+          }
+        }
+      }
+    }
+    stage = stage == S - 1 ? 0 : stage + 1;
+  }
+  if constexpr (KIND == kLayer) {
+    if (!partial) return;
+    constexpr int kTeams = kCta / TEAM, kPitch = kSumPitch<E, TEAM>;
+    float(*acc)[kTeams][E * kPitch] = reinterpret_cast<float(*)[kTeams][E * kPitch]>(shared);
+    copies_wait<0>();  // every copy was waited for where its row was used; the ring is free
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        acc[0][threadIdx.x / TEAM][e * kPitch + lane] = dw[v][e];
+        acc[1][threadIdx.x / TEAM][e * kPitch + lane] = db[v][e];
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < 2 * TEAM * E; i += kCta) {
+        const int which = i / (TEAM * E), c = i % (TEAM * E);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kTeams; ++k) sum += acc[which][k][(c % E) * kPitch + c / E];
+        const int col = TEAM * E * v + c;
+        if (col < t.dim) partial[((int64_t)which * gridDim.x + blockIdx.x) * t.dim + col] = sum;
+      }
+    }
+  }
+}
+
+// Adds the rows of partial [2][slabs][dim] in order: a CTA takes 32 columns of
+// one of the two halves, its 8 warps every eighth row.
+template <typename W>
 __global__ void __launch_bounds__(kThreads)
-forward_kernel(const T* __restrict__ tokens, Rows t, const W* __restrict__ weight,
-               const W* __restrict__ bias, T* __restrict__ out, float* __restrict__ mean,
-               float* __restrict__ rstd, float eps) {
+grad_weight_sum_kernel(const float* __restrict__ partial, int slabs, int dim, W* __restrict__ grad_weight,
+                       W* __restrict__ grad_bias) {
+  __shared__ float acc[kThreads / 32][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  W* to = blockIdx.y ? grad_bias : grad_weight;
+  if (!to) return;
+  const float* from = partial + (int64_t)blockIdx.y * slabs * dim;
+  float sum = 0.f;
+  if (c < dim) {
+#pragma unroll 4
+    for (int s = warp; s < slabs; s += kThreads / 32) sum += from[(int64_t)s * dim + c];
+  }
+  acc[warp][lane] = sum;
+  __syncthreads();
+  if (warp == 0 && c < dim) {
+#pragma unroll
+    for (int w = 1; w < kThreads / 32; ++w) sum += acc[w][lane];
+    to[c] = narrow<W>(sum);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows of more than 4096 elements: one warp per row, several passes over it (the
+// later ones from L1 or L2), the weight's gradient by a kernel of its own.
+// ---------------------------------------------------------------------------
+template <typename T, int KIND>
+__global__ void __launch_bounds__(kThreads)
+forward_wide_kernel(const T* __restrict__ tokens, Rows t, Affine weight, Affine bias, T* __restrict__ out,
+                    float* __restrict__ mean, float* __restrict__ rstd, float eps) {
   const int lane = threadIdx.x & 31;
-  const uint32_t warps = gridDim.x * (kThreads / 32);
-  for (uint32_t slot = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); slot < t.n_slots; slot += warps) {
-    const Place p = place_of(t, slot);
-    if (p.to < 0) continue;
-    const T* x = tokens + p.from;
-    T* y = out + p.to * t.dim;
+  const Turn<32> turn(t);
+  Walker here;
+  if (turn.begin < turn.end) here.find(t, turn.begin);
+  for (int32_t row = turn.begin; row < turn.end; ++row) {
+    here.seek(t, row);
+    const T* x = tokens + here.from(t, row);
+    T* y = out + (int64_t)row * t.dim;
     if (KIND == kLayer) {
       float s = 0.f;
       for (int c = lane; c < t.dim; c += 32) s += widen(x[c]);
@@ -118,16 +799,16 @@ forward_kernel(const T* __restrict__ tokens, Rows t, const W* __restrict__ weigh
         const float d = widen(x[c]) - mu;
         ss += d * d;
       }
-      const float r = 1.0f / sqrtf(warp_sum(ss) / t.dim + eps);
+      const float r = rsqrtf(warp_sum(ss) / t.dim + eps);
       for (int c = lane; c < t.dim; c += 32) {
         float h = (widen(x[c]) - mu) * r;
-        if (weight) h *= widen(weight[c]);
-        if (bias) h += widen(bias[c]);
+        if (weight.p) h *= weight.at<T>(c);
+        if (bias.p) h += bias.at<T>(c);
         y[c] = narrow<T>(h);
       }
       if (mean && lane == 0) {
-        mean[p.to] = mu;
-        rstd[p.to] = r;
+        mean[row] = mu;
+        rstd[row] = r;
       }
     } else {
       float ss = 0.f, top = 0.f;
@@ -137,51 +818,54 @@ forward_kernel(const T* __restrict__ tokens, Rows t, const W* __restrict__ weigh
         top = fmaxf(top, fabsf(v));
       }
       ss = warp_sum(ss);
-      top = warp_max(top);
-      const bool scaled = squares_out_of_range(ss) && top > 0.f && top < INFINITY;
-      if (scaled) {
-        ss = 0.f;
-        for (int c = lane; c < t.dim; c += 32) {
-          const float v = widen(x[c]) / top;
-          ss += v * v;
+      UnitScale u{1.0f, rsqrtf(ss), false};
+      if (!plain_square(ss, least_square(eps))) {
+        top = warp_max(top);
+        if (top > 0.f && top < INFINITY) {
+          ss = 0.f;
+          for (int c = lane; c < t.dim; c += 32) {
+            const float v = widen(x[c]) / top;
+            ss += v * v;
+          }
+          ss = warp_sum(ss);
         }
-        ss = warp_sum(ss);
+        u = unit_scale(ss, top, eps);
       }
-      const UnitScale u = unit_scale(ss, top, scaled, eps);
       for (int c = lane; c < t.dim; c += 32) y[c] = narrow<T>(widen(x[c]) * u.pre * u.inv);
     }
   }
 }
 
-// grad_tokens.  One warp per row; the gradient of a padding row is zero.
-template <typename T, typename W, int KIND>
+// grad_tokens.  One warp per row.
+template <typename T, int KIND>
 __global__ void __launch_bounds__(kThreads)
-backward_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, Rows t,
-                const W* __restrict__ weight, const float* __restrict__ mean,
-                const float* __restrict__ rstd, T* __restrict__ grad_tokens, float eps) {
+backward_wide_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, Rows t, Affine weight,
+                     const float* __restrict__ mean, const float* __restrict__ rstd,
+                     T* __restrict__ grad_tokens, float eps) {
   const int lane = threadIdx.x & 31;
-  const uint32_t warps = gridDim.x * (kThreads / 32);
-  for (uint32_t slot = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); slot < t.n_slots; slot += warps) {
-    const Place p = place_of(t, slot);
-    T* dx = grad_tokens + (int64_t)slot * t.dim;
-    if (p.to < 0) {
-      for (int c = lane; c < t.dim; c += 32) dx[c] = narrow<T>(0.f);
-      continue;
-    }
-    const T* x = tokens + p.from;
-    const T* g = grad + p.to * t.dim;
+  const Turn<32> turn(t);
+  Walker here;
+  if (t.offsets)
+    zero_padding<T, 1>(t, grad_tokens, (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5),
+                       (int64_t)gridDim.x * (kThreads / 32), lane, 32);
+  if (turn.begin < turn.end) here.find(t, turn.begin);
+  for (int32_t row = turn.begin; row < turn.end; ++row) {
+    here.seek(t, row);
+    const T* x = tokens + here.from(t, row);
+    const T* g = grad + (int64_t)row * t.dim;
+    T* dx = grad_tokens + here.slot(t, row) * t.dim;
     if (KIND == kLayer) {
-      const float mu = mean[p.to], r = rstd[p.to];
+      const float mu = mean[row], r = rstd[row];
       float su = 0.f, suh = 0.f;
       for (int c = lane; c < t.dim; c += 32) {
-        const float u = widen(g[c]) * (weight ? widen(weight[c]) : 1.0f);
+        const float u = widen(g[c]) * (weight.p ? weight.at<T>(c) : 1.0f);
         su += u;
         suh += u * ((widen(x[c]) - mu) * r);
       }
       su = warp_sum(su) / t.dim;
       suh = warp_sum(suh) / t.dim;
       for (int c = lane; c < t.dim; c += 32) {
-        const float u = widen(g[c]) * (weight ? widen(weight[c]) : 1.0f);
+        const float u = widen(g[c]) * (weight.p ? weight.at<T>(c) : 1.0f);
         dx[c] = narrow<T>(r * (u - su - (widen(x[c]) - mu) * r * suh));
       }
     } else {
@@ -194,19 +878,21 @@ backward_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, Rows t
       }
       ss = warp_sum(ss);
       xg = warp_sum(xg);
-      top = warp_max(top);
-      const bool scaled = squares_out_of_range(ss) && top > 0.f && top < INFINITY;
-      if (scaled) {
-        ss = xg = 0.f;
-        for (int c = lane; c < t.dim; c += 32) {
-          const float v = widen(x[c]) / top;
-          ss += v * v;
-          xg += v * widen(g[c]);
+      UnitScale u{1.0f, rsqrtf(ss), false};
+      if (!plain_square(ss, least_square(eps))) {
+        top = warp_max(top);
+        if (top > 0.f && top < INFINITY) {
+          ss = xg = 0.f;
+          for (int c = lane; c < t.dim; c += 32) {
+            const float v = widen(x[c]) / top;
+            ss += v * v;
+            xg += v * widen(g[c]);
+          }
+          ss = warp_sum(ss);
+          xg = warp_sum(xg);
         }
-        ss = warp_sum(ss);
-        xg = warp_sum(xg);
+        u = unit_scale(ss, top, eps);
       }
-      const UnitScale u = unit_scale(ss, top, scaled, eps);
       const float along = u.clamped ? 0.0f : xg * u.inv;  // y . g
       for (int c = lane; c < t.dim; c += 32) {
         const float h = widen(x[c]) * u.pre * u.inv;
@@ -217,39 +903,27 @@ backward_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, Rows t
 }
 
 // Partial sums of grad_weight and grad_bias: thread = one column of one slab
-// of rows; slab s covers slots s, s + slabs, ...  partial [2][slabs][dim].
+// of consecutive rows.  partial [2][slabs][dim].
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-grad_weight_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, Rows t,
-                   const float* __restrict__ mean, const float* __restrict__ rstd,
-                   float* __restrict__ partial, int slabs) {
+grad_weight_wide_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, Rows t,
+                        const float* __restrict__ mean, const float* __restrict__ rstd,
+                        float* __restrict__ partial, int slabs) {
   const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= t.dim) return;
+  const int64_t used = t.used(), share = (used + slabs - 1) / slabs;
+  const int32_t begin = (int32_t)min(blockIdx.y * share, used), end = (int32_t)min(begin + share, used);
   float dw = 0.f, db = 0.f;
-  for (uint32_t slot = blockIdx.y; slot < t.n_slots; slot += slabs) {
-    const Place p = place_of(t, slot);
-    if (p.to < 0) continue;
-    const float g = widen(grad[p.to * t.dim + c]);
-    dw += g * ((widen(tokens[p.from + c]) - mean[p.to]) * rstd[p.to]);
+  Walker here;
+  if (begin < end) here.find(t, begin);
+  if (c >= t.dim) return;
+  for (int32_t row = begin; row < end; ++row) {
+    here.seek(t, row);
+    const float g = widen(grad[(int64_t)row * t.dim + c]);
+    dw += g * ((widen(tokens[here.from(t, row) + c]) - mean[row]) * rstd[row]);
     db += g;
   }
   partial[(int64_t)blockIdx.y * t.dim + c] = dw;
   partial[((int64_t)slabs + blockIdx.y) * t.dim + c] = db;
-}
-
-template <typename W>
-__global__ void __launch_bounds__(kThreads)
-grad_weight_sum_kernel(const float* __restrict__ partial, int slabs, int dim, W* __restrict__ grad_weight,
-                       W* __restrict__ grad_bias) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= dim) return;
-  float dw = 0.f, db = 0.f;
-  for (int s = 0; s < slabs; ++s) {
-    dw += partial[(int64_t)s * dim + c];
-    db += partial[((int64_t)slabs + s) * dim + c];
-  }
-  if (grad_weight) grad_weight[c] = narrow<W>(dw);
-  if (grad_bias) grad_bias[c] = narrow<W>(db);
 }
 
 }  // namespace norm

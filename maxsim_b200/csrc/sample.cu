@@ -1,0 +1,42 @@
+// extern "C" entry point of the sampling operator.
+#include "host.h"
+#include "sample.cuh"
+
+using namespace maxsim;
+
+extern "C" {
+
+int maxsim_b200_sample_rows(const float* scores, int64_t score_stride, const float* uniforms,
+                            int64_t uniform_stride, int64_t rows, int64_t cols, int64_t n, double temperature,
+                            const float* temperature_rows, int64_t top_k, const int32_t* top_k_rows, double top_p,
+                            const float* top_p_rows, double min_p, const float* min_p_rows, int64_t* indices,
+                            float* probabilities, void* stream) {
+  if (rows < 0 || cols < 0 || n < 0 || n > cols) return fail(MAXSIM_EINVAL, "need rows >= 0 and 0 <= n <= cols");
+  if (rows >= (1ll << 31)) return fail(MAXSIM_EINVAL, "too many rows");
+  if (cols > (1 << 20)) return fail(MAXSIM_EUNSUPPORTED, "at most 2^20 columns per row; got %lld", (long long)cols);
+  if (n > 1024) return fail(MAXSIM_EUNSUPPORTED, "at most 1024 draws per row; got %lld", (long long)n);
+  if (score_stride < 0 || uniform_stride < 0) return fail(MAXSIM_EINVAL, "strides must not be negative");
+  if (!temperature_rows && !(temperature > 0.0)) return fail(MAXSIM_EINVAL, "temperature must be > 0");
+  if (rows == 0 || n == 0) return MAXSIM_OK;
+  if (!scores || !uniforms || !indices || !probabilities) return fail(MAXSIM_EINVAL, "null pointer argument");
+  sample::Args A;
+  A.scores = scores;
+  A.uniforms = uniforms;
+  A.score_stride = score_stride;
+  A.uniform_stride = uniform_stride;
+  A.rows = rows;
+  A.cols = (int)cols;
+  A.n = (int)n;
+  A.temperature = {temperature, temperature_rows};
+  A.top_p = {top_p, top_p_rows};
+  A.min_p = {min_p, min_p_rows};
+  A.top_k = {top_k, top_k_rows};
+  A.shift = 62;
+  for (int64_t c = 1; c < cols; c <<= 1) --A.shift;
+  A.indices = indices;
+  A.probabilities = probabilities;
+  sample::sample_rows_kernel<<<(unsigned)rows, sample::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(A);
+  return launch_check("sample_rows_kernel");
+}
+
+}  // extern "C"

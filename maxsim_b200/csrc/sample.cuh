@@ -34,7 +34,7 @@ template <typename T, typename S>
 struct Param {
   S value;
   const T* rows;
-  __device__ __forceinline__ S at(int64_t row) const { return rows ? (S)__ldg(rows + row) : value; }
+  __device__ __forceinline__ S at(int64_t row) const { return rows ? (S)rows[row] : value; }
 };
 
 struct Args {

@@ -104,8 +104,8 @@ def _check(name: str, tokens, weight, bias, eps) -> None:
         raise RuntimeError(f"{name} must be a CUDA tensor (maxsim_b200 has no CPU path); got device {tokens.device}")
     _v.require_same_device({n: t for n, t in ((name, tokens), ("weight", weight), ("bias", bias))
                             if t is not None})
-    if tokens.numel() // dim >= 2 ** 31:
-        raise ValueError(f"{name} may have at most 2^31 - 1 rows; got shape {tuple(tokens.shape)}")
+    if tokens.numel() // dim > 2 ** 31 - 4096:
+        raise ValueError(f"{name} may have at most 2^31 - 4096 rows; got shape {tuple(tokens.shape)}")
 
 
 def _packed(kind, padded, lengths, weight, bias, eps, total_tokens):

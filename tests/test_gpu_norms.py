@@ -196,7 +196,9 @@ def test_packed_form_equals_pack_then_norm_bit_for_bit():
 @pytest.mark.parametrize("dim", [64, 100, 768, 1100])
 def test_strided_and_unaligned_rows(dim):
     """Slices of a larger batch: skipped leading tokens, a narrower last
-    dimension at an odd offset, transposed leading dimensions, expanded rows."""
+    dimension at an odd offset, transposed leading dimensions, expanded rows.
+    (Not bit for bit the result on a contiguous copy: the width of the loads, and
+    with it the order of a row's sum, follows the alignment.)"""
     base = rows_of((6, 12, dim + 24), torch.bfloat16, dim)
     w = rows_of((dim,), torch.bfloat16, 1)
     g = torch.Generator().manual_seed(0)
@@ -209,10 +211,10 @@ def test_strided_and_unaligned_rows(dim):
         y = maxsim.layer_norm(x, wv)
         dx, = torch.autograd.grad(y, x, gy)
         check_layer(view, wv, None, gy, y, (dx, None, None))
-        assert torch.equal(y, maxsim.layer_norm(view.contiguous(), wv))
         ln = lengths[: view.shape[0]].clamp(max=view.shape[1])
         p, _ = maxsim.pack_unit_norm(view, ln)
-        assert torch.equal(p, maxsim.pack_unit_norm(view.contiguous(), ln)[0])
+        rows = view[(torch.arange(view.shape[1])[None, :] < ln[:, None]).to(DEV)]
+        check_unit(rows, None, p, None)
     unaligned = rows_of((37 * dim + 1,), torch.bfloat16, 7)[1:].view(37, dim)
     check_layer(unaligned, w, None, None, maxsim.layer_norm(unaligned, w), None)
     w_off = rows_of((dim + 1,), torch.bfloat16, 8)[1:]
