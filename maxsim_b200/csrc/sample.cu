@@ -2,6 +2,22 @@
 #include "host.h"
 #include "sample.cuh"
 
+namespace maxsim {
+namespace {
+
+template <int THREADS, bool CACHED>
+int launch_rows(const sample::Args& A, cudaStream_t st) {
+  auto kern = sample::sample_rows_kernel<THREADS, CACHED>;
+  static std::atomic<unsigned char> configured[kMaxDevices];
+  const size_t most = CACHED ? sample::kMostCached * sizeof(float) : 0;
+  if (int rc = ensure_smem(kern, most, configured)) return rc;
+  kern<<<(unsigned)A.rows, THREADS, CACHED ? A.cols * sizeof(float) : 0, st>>>(A);
+  return launch_check("sample_rows_kernel");
+}
+
+}  // namespace
+}  // namespace maxsim
+
 using namespace maxsim;
 
 extern "C" {
@@ -35,8 +51,11 @@ int maxsim_b200_sample_rows(const float* scores, int64_t score_stride, const flo
   for (int64_t c = 1; c < cols; c <<= 1) --A.shift;
   A.indices = indices;
   A.probabilities = probabilities;
-  sample::sample_rows_kernel<<<(unsigned)rows, sample::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(A);
-  return launch_check("sample_rows_kernel");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (cols <= 2048) return launch_rows<256, true>(A, st);
+  if (cols <= 12288) return launch_rows<512, true>(A, st);
+  if (cols <= sample::kMostCached) return launch_rows<1024, true>(A, st);
+  return launch_rows<1024, false>(A, st);
 }
 
 }  // extern "C"
