@@ -53,7 +53,7 @@ int maxsim_b200_sample_rows(const float* scores, int64_t score_stride, const flo
   A.probabilities = probabilities;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (cols <= 2048) return launch_rows<256, true>(A, st);
-  if (cols <= 12288) return launch_rows<512, true>(A, st);
+  if (cols <= 24576) return launch_rows<512, true>(A, st);
   if (cols <= sample::kMostCached) return launch_rows<1024, true>(A, st);
   return launch_rows<1024, false>(A, st);
 }

@@ -16,7 +16,8 @@
 //
 // Which candidates come out hangs on comparisons, so a, w and the race are 64-bit
 // and masses are whole numbers (w * 2^shift), whose sums do not depend
-// on the order they are taken in.
+// on the order they are taken in.  (The total of the kept weights only scales the
+// probabilities: 64-bit floating point, summed in a fixed order.)
 #pragma once
 
 #include <cuda_runtime.h>
@@ -51,13 +52,61 @@ struct Args {
   float* probabilities;
 };
 
-// Order-preserving image of a float; -0 and +0 are equal.
+// The exponent of a candidate, as defined (best: the row's largest score).
+__device__ __forceinline__ double exponent(float v, float best, double T) {
+  return v == best ? 0.0 : ((double)v - (double)best) / T;
+}
+// The functions of 64-bit arithmetic are calls: inlined wherever they are used they
+// made the kernel large enough that a CTA spent much of its time fetching it.
+__device__ __noinline__ unsigned long long mass_of(float v, float best, double inv_T, double scale) {
+  return __double2ull_rn(exp(v == best ? 0.0 : ((double)v - (double)best) * inv_T) * scale);
+}
+__device__ __noinline__ double race_of(float v, float best, double T, float u) {
+  const double r = exponent(v, best, T) - log(-log((double)u));
+  return r < -1e300 ? -1e300 : r;  // a uniform of 0 comes last; NaN stays
+}
+__device__ __noinline__ float share_of(float v, float best, double T, double total) {
+  return (float)(exp(exponent(v, best, T)) / total);
+}
+// Floats in order, as integers; -0 and +0 are one.
 __device__ __forceinline__ uint32_t key_of(float v) {
   const uint32_t b = __float_as_uint(v + 0.0f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
+}
+// The smallest finite score whose weight is at least `weight` (or whose exponent is at least
+// `least`, with weight 0): weights rise with scores, so one comparison of floats
+// decides afterwards.  `guess` is a few roundings away as a number, which near zero can be a great
+// many floats: steps that double, then halving, some 60 tries at the very most.
+__device__ __noinline__ float first_score(float best, double T, double least, double weight, double guess) {
+  const auto holds = [&](uint32_t key) {
+    const double a = exponent(value_of(key), best, T);
+    return weight > 0.0 ? exp(a) >= weight : a >= least;
+  };
+  const uint32_t lowest = key_of(-3.402823466e38f), top = key_of(best);  // holds(top)
+  uint32_t x = guess >= best ? top : guess > -3.4e38 ? key_of(__double2float_ru(guess)) : lowest;
+  uint32_t out = x, in = x;  // !holds(out), holds(in)
+  if (holds(x)) {
+    for (uint32_t step = 1;; step += step) {
+      if (in == lowest) return value_of(in);
+      const uint32_t next = in - lowest <= step ? lowest : in - step;
+      if (!holds(next)) { out = next; break; }
+      in = next;
+    }
+  } else {
+    for (uint32_t step = 1;; step += step) {
+      const uint32_t next = top - out <= step ? top : out + step;
+      if (next == top || holds(next)) { in = next; break; }
+      out = next;
+    }
+  }
+  while (in - out > 1) {
+    const uint32_t mid = out + (in - out) / 2;
+    if (holds(mid)) in = mid; else out = mid;
+  }
+  return value_of(in);
 }
 
 // 2^y to within 6e-9 of its size, for y <= 0: 2^floor(y + 1/2) times the Taylor series of
@@ -87,13 +136,17 @@ struct Most {
   template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a > b ? a : b; }
 };
 
+struct Or {
+  __device__ __forceinline__ int operator()(int a, int b) const { return a | b; }
+};
+
 // A CTA per row.  The row's scores are kept in shared memory (kCached, up to
 // kMostCached columns) or read again from memory for each pass; with the race
 // they are overwritten by its values.
 //
 // A threshold ("the k-th largest", "the last one before the mass reaches p") is found
-// with histograms over a linear map of the values, kBins bins from the largest to
-// the smallest: counts, or exact masses as two 32-bit words (shared-memory atomics of 32 bits are
+// with histograms over a linear map of the scores, kBins bins from the largest to
+// the smallest, of counts or of masses as two 32-bit words (shared-memory atomics of 32 bits are
 // native, and integer sums do not depend on their order).  The bin that holds the threshold is looked at
 // again: its members are ranked against each other when there are at most
 // kListed, else the map zooms into it.  Every zoom separates its largest from its smallest
@@ -102,10 +155,15 @@ struct Most {
 // The race is run twice: in 32 bits over all kept candidates, as lower bounds
 // with the arithmetic's error taken off, whose n-th largest leaves out everything
 // that cannot be among the n best; and in 64 bits for the few that are left.
+//
+// What bounds it: instructions and latency, not memory.  A row is read once, but
+// every element then takes an exponential, two logarithms and a histogram step, and a
+// row goes through some twenty barriers.
 constexpr int kListed = 256;         // members that are ranked against each other
-constexpr int kMostDrawn = 1024;     // draws of a row
-constexpr int kRaced = 1536;         // candidates of a row that are raced in 64 bits
+constexpr int kRaced = 2048;         // candidates of a row that are raced in 64 bits (a power of two)
+constexpr int kFew = 384;            // kept candidates that go to the 64-bit race without the 32-bit one
 constexpr int kMostCached = 40960;   // columns of a row in shared memory
+constexpr int kBatch = 4;            // elements of a thread whose loads are in flight together
 
 template <int THREADS>
 struct Shared {
@@ -114,15 +172,15 @@ struct Shared {
     uint32_t bins[2][kBins];              // low and high words of a histogram
     struct {
       unsigned long long mass[kListed];   // of the ranked members, best first
-      uint32_t key[kListed];
+      float score[kListed];
       int32_t index[kListed];
     } ranked;
     unsigned long long race[kRaced];      // order-preserving images of 64-bit race values
   };
   int32_t list[kRaced];
-  unsigned long long words[2][THREADS / 32];
+  unsigned long long words[2][5][THREADS / 32];
   unsigned long long found_above;
-  uint32_t found_key;
+  float found_score;
   int32_t found_bin, found_index, members;
 };
 
@@ -131,20 +189,35 @@ struct Block {
   Shared<THREADS>& sh;
   int half = 0;
 
-  // One barrier each: the next one uses the other words.
+  // Every thread gets the results over all threads; up to five values at once.  One
+  // barrier: the next call uses the other words.
   template <typename V, typename Op>
-  __device__ __forceinline__ V reduce(V v, Op op) {
-    static_assert(sizeof(V) <= 8, "");
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, off));
-    V* words = reinterpret_cast<V*>(sh.words[half]);
-    half ^= 1;
-    if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = words[threadIdx.x & (THREADS / 32 - 1)];
-#pragma unroll
-    for (int off = THREADS / 64; off > 0; off >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, off));
+  __device__ __forceinline__ static V lanes(V v, Op op, int from) {
+    for (int off = from; off > 0; off >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, off));
     return v;
+  }
+  template <typename V>
+  __device__ __forceinline__ V* slot(int k) const { return reinterpret_cast<V*>(sh.words[half][k]); }
+
+  template <typename V, typename Op, typename... Rest>
+  __device__ __forceinline__ void put(int k, V v, Op op, Rest... rest) {
+    v = lanes(v, op, 16);
+    if ((threadIdx.x & 31) == 0) slot<V>(k)[threadIdx.x >> 5] = v;
+    if constexpr (sizeof...(rest) > 0) put(k + 1, rest...);
+  }
+  template <typename V, typename Op, typename... Rest>
+  __device__ __forceinline__ void get(int k, V& v, Op op, Rest&&... rest) {
+    v = lanes(slot<V>(k)[threadIdx.x & (THREADS / 32 - 1)], op, THREADS / 64);
+    if constexpr (sizeof...(rest) > 0) get(k + 1, rest...);
+  }
+  // reduce(value, op, value, op, ...): the values are replaced by the results.
+  template <typename... Pairs>
+  __device__ __forceinline__ void reduce(Pairs&&... pairs) {
+    static_assert(sizeof...(pairs) <= 10, "five values");
+    put(0, pairs...);
+    __syncthreads();
+    get(0, pairs...);
+    half ^= 1;
   }
   // Sum of the threads before this one.
   __device__ __forceinline__ unsigned long long before(unsigned long long v, unsigned long long* total) {
@@ -155,7 +228,7 @@ struct Block {
       const unsigned long long up = __shfl_up_sync(0xffffffffu, upto, off);
       if (lane >= off) upto += up;
     }
-    unsigned long long* words = sh.words[half];
+    unsigned long long* words = sh.words[half][0];
     half ^= 1;
     if (lane == 31) words[warp] = upto;
     __syncthreads();
@@ -173,7 +246,8 @@ struct Block {
 };
 
 template <int THREADS, bool kCached>
-__global__ void __launch_bounds__(THREADS) sample_rows_kernel(const __grid_constant__ Args A) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+sample_rows_kernel(const __grid_constant__ Args A) {
   using S = Shared<THREADS>;
   constexpr int kBins = S::kBins;
   extern __shared__ float cache[];
@@ -183,63 +257,83 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(const __grid_const
   const int tid = threadIdx.x, C = A.cols, n = A.n;
   const float* const scores = A.scores + row * A.score_stride;
   const float* const uniforms = A.uniforms + row * A.uniform_stride;
-  const double T = A.temperature.at(row);
-
-  // the best candidate (key 0: there is none)
-  uint32_t top = 0;
-#pragma unroll 4
-  for (int i = tid; i < C; i += THREADS) {
-    const float v = scores[i];
-    if (kCached) cache[i] = v;
-    if (v > -INFINITY) top = max(top, key_of(v));
-  }
-  const uint32_t best_key = block.reduce(top, Most());  // and the barrier behind the cache
   int64_t* const indices = A.indices + row * n;
   float* const probabilities = A.probabilities + row * n;
-  if (best_key == 0 || !(T > 0.0)) {
+  const double T = A.temperature.at(row);
+
+  const auto score = [&](int i) { return kCached ? cache[i] : scores[i]; };
+
+  // the largest and the smallest score, and how many there are
+  float best = -INFINITY, least = INFINITY;
+  int some = 0;
+  for (int i0 = tid; i0 < C; i0 += kBatch * THREADS) {
+    float v[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) v[b] = i0 + b * THREADS < C ? scores[i0 + b * THREADS] : -INFINITY;
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (kCached && i0 + b * THREADS < C) cache[i0 + b * THREADS] = v[b];
+      if (v[b] > -INFINITY) {
+        best = fmaxf(best, v[b]);
+        least = fminf(least, v[b]);
+        ++some;
+      }
+    }
+  }
+  block.reduce(best, Most(), least, Least(), some, Add());  // and the barrier behind the cache
+  if (some == 0 || !(T > 0.0)) {
     for (int d = tid; d < n; d += THREADS) {
       indices[d] = -1;
       probabilities[d] = 0.f;
     }
     return;
   }
-  const float best = value_of(best_key);
-  const double best_d = best, inv_T = 1.0 / T;
-  const float inv_Tf = (float)inv_T;
-  const auto score = [&](int i) { return kCached ? cache[i] : scores[i]; };
-  // the exponent, as defined; quickly and to within 1e-6 of its size; for masses
-  const auto exponent = [&](float v) { return v == best ? 0.0 : ((double)v - best_d) / T; };
-  const auto quick = [&](float v) { return v == best ? 0.f : fmaxf(v - best, -3.4e38f) * inv_Tf; };
-  const double scale = ldexp(1.0, A.shift);
-  const auto mass = [&](float v) {
-    return __double2ull_rn(exp(v == best ? 0.0 : ((double)v - best_d) * inv_T) * scale);
-  };
-  const auto candidate = [&](float v) {  // false for NaN and -inf
-    const float a = quick(v);
-    return v > -INFINITY && (a > -699.f || (a > -701.f && exponent(v) >= kLeast));
-  };
+  const double inv_T = 1.0 / T, scale = ldexp(1.0, A.shift);
+  // candidates are the scores from `first` on (false for NaN and -inf)
+  const float first = first_score(best, T, kLeast, 0.0, (double)best + kLeast * T);
 
-  // The filters keep a prefix: keys above `cut`, and those equal to it up to index `cut_index`.
-  uint32_t cut = 0;
+  // The filters keep a prefix: scores above `cut`, and those equal to it up to index `cut_index`.
+  float cut = -INFINITY;
   int32_t cut_index = -1;
-  const auto inside = [&](uint32_t key, int i) { return key > cut || (key == cut && i <= cut_index); };
+  const auto inside = [&](float v, int i) { return v > cut || (v == cut && i <= cut_index); };
 
-  // Moves the cut.  The members are the candidates inside it whose weight is not
-  // zero, of which `lowest` is the smallest key; weight(v) is what they add up, and
-  // the new last member is the last one before which enough(sum) is false.
-  const auto move_cut = [&](uint32_t lowest, auto weight, auto counts, auto enough, auto start) {
-    constexpr bool kCounts = decltype(counts)::value;
-    uint32_t high = best_key, low = lowest;
+  const int64_t k = A.top_k.at(row);
+  const double p = A.top_p.at(row);
+  const bool by_count = k > 0 && k < some, by_mass = p > 0.0 && p < 1.0;
+  if (by_count && least < first) {  // entries that weigh nothing are no candidates
+    least = INFINITY;
+    some = 0;
+    for (int i = tid; i < C; i += THREADS) {
+      const float v = score(i);
+      if (v >= first) {
+        least = fminf(least, v);
+        ++some;
+      }
+    }
+    block.reduce(least, Least(), some, Add());
+  }
+  // Twice the same search: what the members add up to (one each, or their masses) has to
+  // reach `limit`, and the new last member is the last one before which it has not.
+#pragma unroll 1
+  for (int masses = 0; masses < 2; ++masses) {
+    if (masses ? !by_mass : !(by_count && k < some)) continue;
+    double limit = (double)k;
+    float high = best, low = fmaxf(least, first);
+    if (masses) {  // below -(shift + 2) ln 2 a mass rounds to none
+      const float none = best + (-0.6931472f * (A.shift + 2)) * (float)T;
+      low = fminf(fmaxf(fmaxf(low, cut), none), best);
+    }
+    const auto weight = [&](float v) { return masses ? mass_of(v, best, inv_T, scale) : 1ull; };
+    const auto enough = [&](unsigned long long sum) { return !((double)sum < limit); };
     unsigned long long above = 0;
-    bool first = true;
+    bool fresh = true;
     for (;;) {
-      const float v_high = value_of(high);
-      const float spread = v_high - value_of(low);
-      const float per = spread < 3e38f ? (kBins - 1) / spread : 0.f;
-      const auto bin_of = [&](float v) {  // falls with the value; in halves where a difference overflows
-        const float t = per > 0.f ? (v_high - v) * per
-                                  : (0.5f * v_high - 0.5f * v) * ((kBins - 1) / (0.5f * v_high - 0.5f * value_of(low)));
-        return min((int)t, kBins - 1);
+      const auto member = [&](float v, int i) { return v >= low && v <= high && inside(v, i); };
+      // the map falls with the score; in halves where a difference would overflow
+      const float half = high - low < 3e38f ? 1.f : 0.5f;
+      const float per = (kBins - 1) / (half * high - half * low);
+      const auto bin_of = [&](float v) {
+        return low == high ? 0 : min((int)((half * high - half * v) * per), kBins - 1);
       };
       __syncthreads();  // whatever the words of the union held has been read
       for (int i = tid; i < kBins; i += THREADS) sh.bins[0][i] = sh.bins[1][i] = 0;
@@ -247,23 +341,21 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(const __grid_const
       __syncthreads();
       for (int i = tid; i < C; i += THREADS) {
         const float v = score(i);
-        const uint32_t key = key_of(v);
-        if (!candidate(v) || key < low || key > high || !inside(key, i)) continue;
-        const int bin = low == high ? 0 : bin_of(v);
-        if (kCounts) {
-          // lanes of a warp that meet in one bin are added up first
-          const unsigned active = __activemask();
-          int same;
-          __match_all_sync(active, bin, &same);
-          if (!same) atomicAdd(&sh.bins[0][bin], 1u);
-          else if ((tid & 31) == __ffs(active) - 1) atomicAdd(&sh.bins[0][bin], (uint32_t)__popc(active));
-        } else {
+        if (!member(v, i)) continue;
+        const int bin = bin_of(v);
+        if (masses) {
           const unsigned long long w = weight(v);
           if (w) {
             const uint32_t lo = (uint32_t)w, old = atomicAdd(&sh.bins[0][bin], lo);
             const uint32_t up = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
             if (up) atomicAdd(&sh.bins[1][bin], up);
           }
+        } else {  // lanes that all meet in one bin are added up first
+          const unsigned active = __activemask();
+          int same;
+          __match_all_sync(active, bin, &same);
+          if (!same) atomicAdd(&sh.bins[0][bin], 1u);
+          else if ((tid & 31) == __ffs(active) - 1) atomicAdd(&sh.bins[0][bin], (uint32_t)__popc(active));
         }
       }
       __syncthreads();
@@ -272,63 +364,58 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(const __grid_const
       const unsigned long long w1 = sh.bins[0][b0 + 1] + ((unsigned long long)sh.bins[1][b0 + 1] << 32);
       unsigned long long total;
       const unsigned long long pre = above + block.before(w0 + w1, &total);
-      if (first) start(total);  // the weight of all members: what enough() goes by
-      first = false;
-      if (!enough(pre) && enough(pre + w0)) {
-        sh.found_bin = b0;
-        sh.found_above = pre;
-      } else if (!enough(pre + w0) && enough(pre + w0 + w1)) {
-        sh.found_bin = b0 + 1;
-        sh.found_above = pre + w0;
+      if (masses && fresh) limit = p * (double)total;
+      fresh = false;
+      if (!enough(pre) && enough(pre + w0 + w1)) {  // one thread
+        const bool second = !enough(pre + w0);
+        sh.found_bin = b0 + second;
+        sh.found_above = second ? pre + w0 : pre;
       }
       __syncthreads();
       const int bin = sh.found_bin;
       above = sh.found_above;
-      uint32_t most = 0, least = 0xffffffffu;
+      float most = -INFINITY, fewest = INFINITY;
       for (int i = tid; i < C; i += THREADS) {
         const float v = score(i);
-        const uint32_t key = key_of(v);
-        if (!candidate(v) || key < low || key > high || !inside(key, i)) continue;
-        if ((low == high ? 0 : bin_of(v)) != bin) continue;
-        most = max(most, key);
-        least = min(least, key);
+        if (!member(v, i) || bin_of(v) != bin) continue;
+        most = fmaxf(most, v);
+        fewest = fminf(fewest, v);
         const int at = atomicAdd(&sh.members, 1);
         if (at < kListed) sh.list[at] = i;
       }
-      most = block.reduce(most, Most());
-      least = block.reduce(least, Least());
+      block.reduce(most, Most(), fewest, Least());
       const int members = sh.members;
       if (members <= kListed) {
-        uint32_t my_key = 0;
-        int my_index = 0, rank = -1;
-        if (tid < members) {
-          my_index = sh.list[tid];
-          my_key = key_of(score(my_index));
-          sh.ranked.key[tid] = my_key;
-        }
         static_assert(THREADS >= kListed, "a thread per ranked member");
+        float mine = 0.f;
+        int index = 0, rank = 0;
+        if (tid < members) {
+          index = sh.list[tid];
+          mine = score(index);
+          sh.ranked.score[tid] = mine;
+        }
         __syncthreads();
         if (tid < members) {
-          rank = 0;
+#pragma unroll 1
           for (int j = 0; j < members; ++j) {
-            const uint32_t k = sh.ranked.key[j];
-            rank += k > my_key || (k == my_key && sh.list[j] < my_index);
+            const float v = sh.ranked.score[j];
+            rank += v > mine || (v == mine && sh.list[j] < index);
           }
         }
         __syncthreads();
-        if (rank >= 0) {
-          sh.ranked.key[rank] = my_key;
-          sh.ranked.index[rank] = my_index;
-          sh.ranked.mass[rank] = kCounts ? 1ull : weight(value_of(my_key));
+        if (tid < members) {
+          sh.ranked.score[rank] = mine;
+          sh.ranked.index[rank] = index;
+          sh.ranked.mass[rank] = weight(mine);
         }
         __syncthreads();
         if (tid < 32) {  // the last member before which the sum is not enough
           unsigned long long sum = above;
           int last = 0;
+#pragma unroll 1
           for (int base = 0; base < members; base += 32) {
             const unsigned long long w = base + tid < members ? sh.ranked.mass[base + tid] : 0;
             unsigned long long upto = w;
-#pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
               const unsigned long long up = __shfl_up_sync(0xffffffffu, upto, off);
               if (tid >= off) upto += up;
@@ -339,18 +426,18 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(const __grid_const
             sum += __shfl_sync(0xffffffffu, upto, 31);
           }
           if (tid == 0) {
-            sh.found_key = sh.ranked.key[last];
+            sh.found_score = sh.ranked.score[last];
             sh.found_index = sh.ranked.index[last];
           }
         }
         __syncthreads();
-        cut = sh.found_key;
+        cut = sh.found_score;
         cut_index = sh.found_index;
-        return;
+        break;
       }
-      if (most == least) {
+      if (most == fewest) {
         // More equal members than are listed: how many stay, and the index of the last of them.
-        const unsigned long long each = kCounts ? 1ull : weight(value_of(most));
+        const unsigned long long each = weight(most);
         int lo = 1, hi = members;  // the largest r with !enough(above + (r - 1) * each)
         while (lo < hi) {
           const int mid = lo + (hi - lo + 1) / 2;
@@ -359,167 +446,174 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(const __grid_const
         int from = 0, to = C - 1;  // the smallest index up to which there are lo of them
         while (from < to) {
           const int mid = from + (to - from) / 2;
-          int some = 0;
+          int equal = 0;
           for (int i = tid; i <= mid; i += THREADS) {
             const float v = score(i);
-            some += candidate(v) && key_of(v) == most && inside(most, i);
+            equal += v == most && inside(v, i);
           }
-          if (block.reduce(some, Add()) >= lo) to = mid; else from = mid + 1;
+          block.reduce(equal, Add());
+          if (equal >= lo) to = mid; else from = mid + 1;
         }
         cut = most;
         cut_index = from;
-        return;
+        break;
       }
       high = most;
-      low = least;
+      low = fewest;
     }
-  };
-
-  const int64_t k = A.top_k.at(row);
-  const double p = A.top_p.at(row);
-  const bool by_mass = p > 0.0 && p < 1.0;
-  if (k > 0 && k < C) {
-    uint32_t least = 0xffffffffu;
-    int some = 0;
-    for (int i = tid; i < C; i += THREADS) {
-      const float v = score(i);
-      if (!candidate(v)) continue;
-      least = min(least, key_of(v));
-      ++some;
-    }
-    least = block.reduce(least, Least());
-    some = block.reduce(some, Add());
-    if (k < some) {
-      const unsigned long long want = (unsigned long long)k;
-      move_cut(least, [](float) { return 1ull; }, std::true_type(),
-               [&](unsigned long long sum) { return sum >= want; }, [](unsigned long long) {});
-    }
-  }
-  if (by_mass) {
-    // the smallest member with a mass: below -(shift + 2) ln 2 a weight rounds to none
-    const float none = -0.6931472f * (A.shift + 2);
-    uint32_t least = 0xffffffffu;
-    for (int i = tid; i < C; i += THREADS) {
-      const float v = score(i);
-      if (candidate(v) && quick(v) > none && inside(key_of(v), i)) least = min(least, key_of(v));
-    }
-    least = block.reduce(least, Least());
-    double limit = 0.0;
-    move_cut(least, mass, std::false_type(), [&](unsigned long long sum) { return !((double)sum < limit); },
-             [&](unsigned long long total) { limit = p * (double)total; });
   }
   const double least_share = A.min_p.at(row);
   const bool by_share = least_share > 0.0 && least_share <= 1.0;
-  const float share_exponent = by_share ? (float)log(least_share) : -INFINITY;
-  const float share_margin = 1e-5f * (1.f - share_exponent);
-  const auto kept = [&](float v, int i) {
-    if (!candidate(v) || !inside(key_of(v), i)) return false;
-    if (!by_share) return true;
-    const float d = quick(v) - share_exponent;
-    return d > share_margin || (d > -share_margin && exp(exponent(v)) >= least_share);
-  };
+  const float floor_score =
+      by_share ? fmaxf(first, first_score(best, T, 0.0, least_share, (double)best + T * log(least_share))) : first;
+  const auto kept = [&](float v, int i) { return v >= floor_score && inside(v, i); };
 
-  // The race in 32 bits: lower bounds.  a and the logarithms are off by at most a few
-  // 2^-23 of their size, and the size of either is at most |sum| + 36 (a uniform
-  // strictly between 0 and 1 has -4.7 < -log(-log u) < 16.7).
-  const auto error_at = [](float g) { return 1e-6f * (fabsf(g) + 40.f); };
-  const auto lower_race = [&](float v, float u) {
-    const float g = quick(v) - logf(-logf(u));
-    return g - error_at(g);
+  // The race in 32 bits: lower bounds.  a is off by a few 2^-24 of its size, the outer
+  // logarithm by 2^-21; with -4.7 < -log(-log u) < 16.7 for a uniform strictly between 0
+  // and 1 the size of either is at most |sum| + 17.
+  const float inv_Tf = (float)inv_T;
+  const auto lower = [&](float v, float u) {
+    const float g = (v == best ? 0.f : fmaxf(v - best, -3.4e38f) * inv_Tf) - __logf(-logf(u));
+    return g - 1e-6f * (fabsf(g) + 40.f);
   };
-  const bool exact_sum = k > 0 || by_mass;  // few are kept: the masses that the filters saw
+  const bool filtered = by_count || by_mass || by_share;
   const double per_bit = inv_T * 1.4426950408889634;
-  unsigned long long sum = 0;
+  double total = 0.0;
   float g_most = -INFINITY, g_least = INFINITY;
   int open = 0, odd = 0;  // candidates in the race; uniforms of 0 and 1
-  for (int i = tid; i < C; i += THREADS) {
-    const float v = score(i);
-    float g = -INFINITY;
-    if (kept(v, i)) {
-      sum += exact_sum ? mass(v) : v == best ? (unsigned long long)scale
-                                             : __double2ull_rn(exp2_short(((double)v - best_d) * per_bit) * scale);
-      const float u = uniforms[i];
-      if (u > 0.f && u < 1.f) {
-        g = lower_race(v, u);
-        g_most = fmaxf(g_most, g);
-        g_least = fminf(g_least, g);
-        ++open;
-      } else if (u == 0.f || u == 1.f) {
-        odd |= u == 1.f ? 2 : 1;
-      }
+  __syncthreads();
+  if (tid == 0) sh.members = 0;
+  __syncthreads();
+  for (int i0 = tid; i0 < C; i0 += 2 * THREADS) {
+    float v[2], u[2];
+    bool in[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int i = i0 + b * THREADS;
+      v[b] = i < C ? score(i) : -INFINITY;
+      in[b] = kept(v[b], i);
+      u[b] = in[b] ? uniforms[i] : 0.f;
     }
-    if (kCached) cache[i] = g;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int i = i0 + b * THREADS;
+      float g = -INFINITY;
+      if (in[b]) {
+        total += v[b] == best ? 1.0 : exp2_short(((double)v[b] - (double)best) * per_bit);
+        if (u[b] > 0.f && u[b] < 1.f) {
+          g = lower(v[b], u[b]);
+          g_most = fmaxf(g_most, g);
+          g_least = fminf(g_least, g);
+          ++open;
+          if (filtered) {
+            const int at = atomicAdd(&sh.members, 1);
+            if (at < kFew) sh.list[at] = i;
+          }
+        } else if (u[b] == 0.f || u[b] == 1.f) {
+          odd |= u[b] == 1.f ? 2 : 1;
+        }
+      }
+      if (kCached && i < C) cache[i] = g;
+    }
   }
-  const double total = (double)block.reduce(sum, Add());
-  g_most = block.reduce(g_most, Most());
-  g_least = block.reduce(g_least, Least());
-  open = block.reduce(open, Add());
-  odd = block.reduce(odd, [](int a, int b) { return a | b; });
-  const auto race = [&](int i) {
-    const float v = scores[i];
-    const double r = exponent(v) - log(-log((double)uniforms[i]));
-    return r < -1e300 ? -1e300 : r;  // a uniform of 0 comes last; NaN stays
-  };
-  const auto share = [&](int i) { return (float)(exp(exponent(scores[i])) * scale / total); };
+  block.reduce(total, Add(), g_most, Most(), g_least, Least(), open, Add(), odd, Or());
 
   bool listed = !(odd & 2) && (open >= n || !(odd & 1));
   if (listed && open > 0) {
-    const float g_spread = g_most - g_least;
-    const float per = g_spread > 0.f ? (kBins - 1) / g_spread : 0.f;
-    const auto bin_of = [&](float g) { return max(0, min((int)((g_most - g) * per), kBins - 1)); };
-    const auto bound = [&](int i) {
-      if (kCached) return cache[i];
-      const float v = score(i), u = uniforms[i];
-      return kept(v, i) && u > 0.f && u < 1.f ? lower_race(v, u) : -INFINITY;
-    };
-    __syncthreads();
-    if (tid == 0) {
-      sh.members = 0;
-      sh.found_bin = kBins - 1;
-    }
-    if (open > n) {
-      for (int i = tid; i < kBins; i += THREADS) sh.bins[0][i] = 0;
+    int members = open;
+    if (!filtered || open > kFew) {
+      const float per = g_most > g_least ? (kBins - 1) / (g_most - g_least) : 0.f;
+      const auto bound = [&](int i) {
+        if (kCached) return cache[i];
+        const float v = scores[i], u = uniforms[i];
+        return kept(v, i) && u > 0.f && u < 1.f ? lower(v, u) : -INFINITY;
+      };
+      float edge = g_least;  // at least n lower bounds reach it
+      __syncthreads();
+      if (tid == 0) sh.members = 0;
+      if (open > n) {
+        for (int i = tid; i < kBins; i += THREADS) sh.bins[0][i] = 0;
+        __syncthreads();
+        for (int i = tid; i < C; i += THREADS) {
+          const float g = bound(i);
+          if (g > -INFINITY) atomicAdd(&sh.bins[0][min((int)((g_most - g) * per), kBins - 1)], 1u);
+        }
+        __syncthreads();
+        const unsigned long long c0 = sh.bins[0][2 * tid], c1 = sh.bins[0][2 * tid + 1];
+        unsigned long long all;
+        const unsigned long long pre = block.before(c0 + c1, &all), want = n;
+        if (pre < want && pre + c0 + c1 >= want) sh.found_bin = 2 * tid + (pre + c0 < want);
+        __syncthreads();
+        // the lower end of the bin, a hundredth of its width and a rounding of the sum beyond it
+        if (sh.found_bin < kBins - 1 && per > 0.f)
+          edge = fmaxf(edge, g_most - (sh.found_bin + 1.01f) / per - 4e-7f * (fabsf(g_most) + fabsf(g_least)));
+      }
+      edge -= 2.1e-6f * (fabsf(edge) + 41.f);  // what an upper bound may lie above its lower one
       __syncthreads();
       for (int i = tid; i < C; i += THREADS) {
-        const float g = bound(i);
-        if (g > -INFINITY) atomicAdd(&sh.bins[0][bin_of(g)], 1u);
-      }
-      __syncthreads();
-      const unsigned long long c0 = sh.bins[0][2 * tid], c1 = sh.bins[0][2 * tid + 1];
-      unsigned long long all;
-      const unsigned long long pre = block.before(c0 + c1, &all), want = n;
-      if (pre < want && pre + c0 >= want) sh.found_bin = 2 * tid;
-      else if (pre + c0 < want && pre + c0 + c1 >= want) sh.found_bin = 2 * tid + 1;
-    }
-    __syncthreads();
-    const int bin = sh.found_bin;
-    for (int i = tid; i < C; i += THREADS) {
-      const float g = bound(i);
-      if (g > -INFINITY && bin_of(g + 2.01f * error_at(g)) <= bin) {
+        if (bound(i) < edge) continue;
         const int at = atomicAdd(&sh.members, 1);
         if (at < kRaced) sh.list[at] = i;
       }
+      __syncthreads();
+      members = sh.members;
     }
-    __syncthreads();
-    const int members = sh.members;
     listed = members <= kRaced;
     if (listed) {
+#pragma unroll 1
       for (int j = tid; j < members; j += THREADS) {
-        const unsigned long long bits = (unsigned long long)__double_as_longlong(race(sh.list[j]) + 0.0);
+        const int i = sh.list[j];
+        const double r = race_of(scores[i], best, T, uniforms[i]) + 0.0;  // -0 as 0
+        const unsigned long long bits = (unsigned long long)__double_as_longlong(r);
         sh.race[j] = bits >> 63 ? ~bits : bits | (1ull << 63);
       }
       __syncthreads();
-      for (int j = tid; j < members; j += THREADS) {
-        const unsigned long long mine = sh.race[j];
-        const int i = sh.list[j];
-        int rank = 0;
-        for (int o = 0; o < members; ++o) {
-          const unsigned long long other = sh.race[o];
-          rank += other > mine || (other == mine && sh.list[o] < i);
+      if (members <= kListed) {  // ranked against each other
+        if (tid < members) {
+          const unsigned long long mine = sh.race[tid];
+          const int i = sh.list[tid];
+          int rank = 0;
+#pragma unroll 2
+          for (int o = 0; o < members; ++o) {
+            const unsigned long long other = sh.race[o];
+            rank += other > mine || (other == mine && sh.list[o] < i);
+          }
+          if (rank < n) {
+            indices[rank] = i;
+            probabilities[rank] = share_of(scores[i], best, T, total);
+          }
         }
-        if (rank < n) {
-          indices[rank] = i;
-          probabilities[rank] = share(i);
+      } else {  // sorted, best first
+        int size = 2 * kListed;
+        while (size < members) size *= 2;
+        for (int j = members + tid; j < size; j += THREADS) {
+          sh.race[j] = 0;
+          sh.list[j] = 0x7fffffff;
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int span = 2; span <= size; span <<= 1) {
+#pragma unroll 1
+          for (int gap = span >> 1; gap > 0; gap >>= 1) {
+#pragma unroll 1
+            for (int q = tid; q < size / 2; q += THREADS) {
+              const int a = ((q & ~(gap - 1)) << 1) | (q & (gap - 1)), b = a | gap;
+              const unsigned long long ra = sh.race[a], rb = sh.race[b];
+              const int ia = sh.list[a], ib = sh.list[b];
+              const bool b_first = rb > ra || (rb == ra && ib < ia);
+              if (b_first == ((a & span) == 0)) {
+                sh.race[a] = rb;
+                sh.race[b] = ra;
+                sh.list[a] = ib;
+                sh.list[b] = ia;
+              }
+            }
+            __syncthreads();
+          }
+        }
+        for (int d = tid; d < min(n, members); d += THREADS) {
+          indices[d] = sh.list[d];
+          probabilities[d] = share_of(scores[sh.list[d]], best, T, total);
         }
       }
       for (int d = members + tid; d < n; d += THREADS) {
@@ -534,13 +628,15 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(const __grid_const
   double last = INFINITY;
   int last_index = -1;
   bool more = true;
+#pragma unroll 1
   for (int d = 0; d < n; ++d) {
     double g = -INFINITY;
     int at = C;
     if (more) {
+#pragma unroll 1
       for (int i = tid; i < C; i += THREADS) {
         if (!kept(scores[i], i)) continue;
-        const double r = race(i);
+        const double r = race_of(scores[i], best, T, uniforms[i]);
         if (!(r >= -1e300) || r > last || (r == last && i <= last_index)) continue;
         if (r > g) {
           g = r;
@@ -548,14 +644,16 @@ __global__ void __launch_bounds__(THREADS) sample_rows_kernel(const __grid_const
         }
       }
     }
-    const double most = block.reduce(g, Most());
-    const int first = block.reduce(g == most && most > -INFINITY ? at : C, Least());
-    more = first < C;
+    double most = g;
+    block.reduce(most, Most());
+    if (g != most || !(most > -INFINITY)) at = C;
+    block.reduce(at, Least());
+    more = at < C;
     last = most;
-    last_index = first;
+    last_index = at;
     if (tid == 0) {
-      indices[d] = more ? first : -1;
-      probabilities[d] = more ? share(first) : 0.f;
+      indices[d] = more ? at : -1;
+      probabilities[d] = more ? share_of(scores[at], best, T, total) : 0.f;
     }
   }
 }
