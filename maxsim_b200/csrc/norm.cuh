@@ -20,6 +20,8 @@
 
 #include <type_traits>
 
+#include "async.cuh"
+
 namespace maxsim {
 namespace norm {
 
@@ -280,20 +282,6 @@ constexpr int kBackwardBytes = [] {
   const int sums = KIND == kLayer ? kSumBytes<E, TEAM> : 0;
   return ring > sums ? ring : sums;
 }();
-
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* shared, const void* global) {
-  const uint32_t to = (uint32_t)__cvta_generic_to_shared(shared);
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(global) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(global) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
-}
 
 // Sums over a team.  Teams of one warp or less use shuffles: all lanes of the
 // warp take part, whether their row counts or not.  A CTA team takes one

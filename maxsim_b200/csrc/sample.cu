@@ -1,3 +1,4 @@
+#include <stdlib.h>
 // extern "C" entry point of the sampling operator.
 #include "host.h"
 #include "sample.cuh"
@@ -49,9 +50,11 @@ int maxsim_b200_sample_rows(const float* scores, int64_t score_stride, const flo
   A.top_k = {top_k, top_k_rows};
   A.shift = 62;
   for (int64_t c = 1; c < cols; c <<= 1) --A.shift;
+  if (A.shift > 51) A.shift = 51;
   A.indices = indices;
   A.probabilities = probabilities;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (getenv("MS_T") && cols <= 2048) { int q = atoi(getenv("MS_T")); if (q==512) return launch_rows<512, true>(A, st); if (q==128) return launch_rows<128, true>(A, st);}
   if (cols <= 2048) return launch_rows<256, true>(A, st);
   if (cols <= 24576) return launch_rows<512, true>(A, st);
   if (cols <= sample::kMostCached) return launch_rows<1024, true>(A, st);

@@ -24,7 +24,7 @@
 #include <math.h>
 #include <stdint.h>
 
-#include <type_traits>
+#include "async.cuh"
 
 namespace maxsim {
 namespace sample {
@@ -56,10 +56,43 @@ struct Args {
 __device__ __forceinline__ double exponent(float v, float best, double T) {
   return v == best ? 0.0 : ((double)v - (double)best) / T;
 }
-// The functions of 64-bit arithmetic are calls: inlined wherever they are used they
+// 2^y for -1010 < y <= 0, as 2^n times the Taylor series of 2^f = e^(f ln 2) up to f^DEGREE, n the
+// whole number next to y and |f| <= 1/2.  The first term left out is below 6e-9 for degree 7 and
+// 3e-13 for degree 10.  n comes out of the low bits of y + 1.5 * 2^52 and goes into the
+// exponent's, with `more` added to it.
+template <int DEGREE>
+__device__ __forceinline__ double exp2_series(double y, int more) {
+  constexpr double c[11] = {1.0,
+                            0.6931471805599453,
+                            0.2402265069591007,
+                            0.055504108664821576,
+                            0.009618129107628477,
+                            0.0013333558146428441,
+                            0.00015403530393381606,
+                            1.5252733804059838e-05,
+                            1.3215486790144305e-06,
+                            1.0178086009239696e-07,
+                            7.054911620801121e-09};
+  const double whole = y + 6755399441055744.0, f = y - (whole - 6755399441055744.0);
+  double e = c[DEGREE];
+#pragma unroll
+  for (int k = DEGREE - 1; k >= 0; --k) e = e * f + c[k];
+  return __hiloint2double(__double2hiint(e) + ((__double2loint(whole) + more) << 20), __double2loint(e));
+}
+// An infinite score as a finite one: only the difference of two scores counts, and where
+// the best is infinite every candidate is.
+__device__ __forceinline__ double finite(float v) { return (double)fminf(v, 3.402823466e38f); }
+
+// w * 2^shift as a whole number (shift <= 51), per_bit = 1 / (T ln 2); v not so far below the best
+// that w < 2^-900.
+__device__ __forceinline__ unsigned long long mass_here(float v, double best, double per_bit, int shift) {
+  const double m = exp2_series<10>((finite(v) - best) * per_bit, shift) + 4503599627370496.0;  // 2^52: rounds
+  return (unsigned long long)__double_as_longlong(m) & 0xfffffffffffffull;
+}
+// The functions of more 64-bit arithmetic are calls: inlined wherever they are used they
 // made the kernel large enough that a CTA spent much of its time fetching it.
-__device__ __noinline__ unsigned long long mass_of(float v, float best, double inv_T, double scale) {
-  return __double2ull_rn(exp(v == best ? 0.0 : ((double)v - (double)best) * inv_T) * scale);
+__device__ __noinline__ unsigned long long mass_of(float v, double best, double per_bit, int shift) {
+  return mass_here(v, best, per_bit, shift);
 }
 __device__ __noinline__ double race_of(float v, float best, double T, float u) {
   const double r = exponent(v, best, T) - log(-log((double)u));
@@ -109,23 +142,6 @@ __device__ __noinline__ float first_score(float best, double T, double least, do
   return value_of(in);
 }
 
-// 2^y to within 6e-9 of its size, for y <= 0: 2^floor(y + 1/2) times the Taylor series of
-// e^r at r = ln 2 (y - floor(y + 1/2)), |r| <= 0.3466, cut after r^7 / 7! (the next
-// term is 0.3466^8 / 8! = 5.2e-9).  About a third of the 64-bit operations of exp().
-__device__ __forceinline__ double exp2_short(double y) {
-  y = y < -1000.0 ? -1000.0 : y;
-  const double n = floor(y + 0.5), r = (y - n) * 0.6931471805599453;
-  double e = 1.0 / 5040;
-  e = e * r + 1.0 / 720;
-  e = e * r + 1.0 / 120;
-  e = e * r + 1.0 / 24;
-  e = e * r + 1.0 / 6;
-  e = e * r + 0.5;
-  e = e * r + 1.0;
-  e = e * r + 1.0;
-  return e * __longlong_as_double((long long)((int)n + 1023) << 52);
-}
-
 struct Add {
   template <typename V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
 };
@@ -159,7 +175,6 @@ struct Or {
 // What bounds it: instructions and latency, not memory.  A row is read once, but
 // every element then takes an exponential, two logarithms and a histogram step, and a
 // row goes through some twenty barriers.
-constexpr int kListed = 256;         // members that are ranked against each other
 constexpr int kRaced = 2048;         // candidates of a row that are raced in 64 bits (a power of two)
 constexpr int kFew = 384;            // kept candidates that go to the 64-bit race without the 32-bit one
 constexpr int kMostCached = 40960;   // columns of a row in shared memory
@@ -168,6 +183,7 @@ constexpr int kBatch = 4;            // elements of a thread whose loads are in 
 template <int THREADS>
 struct Shared {
   static constexpr int kBins = 2 * THREADS;
+  static constexpr int kListed = THREADS < 256 ? THREADS : 256;  // members that are ranked against each other
   union {
     uint32_t bins[2][kBins];              // low and high words of a histogram
     struct {
@@ -249,7 +265,7 @@ template <int THREADS, bool kCached>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 sample_rows_kernel(const __grid_constant__ Args A) {
   using S = Shared<THREADS>;
-  constexpr int kBins = S::kBins;
+  constexpr int kBins = S::kBins, kListed = S::kListed;
   extern __shared__ float cache[];
   __shared__ S sh;
   Block<THREADS> block{sh};
@@ -263,16 +279,31 @@ sample_rows_kernel(const __grid_constant__ Args A) {
 
   const auto score = [&](int i) { return kCached ? cache[i] : scores[i]; };
 
+  // The row comes into shared memory with everything in flight at once; its uniforms, needed
+  // several passes later, are asked into L2 meanwhile.
+  if (kCached) {
+    if (((uintptr_t)scores & 15) == 0) {
+      for (int i = 4 * tid; i + 3 < C; i += 4 * THREADS) copy_async<16>(cache + i, scores + i);
+      for (int i = (C & ~3) + tid; i < C; i += THREADS) copy_async<4>(cache + i, scores + i);
+    } else {
+      for (int i = tid; i < C; i += THREADS) copy_async<4>(cache + i, scores + i);
+    }
+    copies_commit();
+  }
+  for (int i = 32 * tid; i < C; i += 32 * THREADS) asm volatile("prefetch.global.L2 [%0];" ::"l"(uniforms + i));
+  if (kCached) {
+    copies_wait<0>();
+    __syncthreads();
+  }
   // the largest and the smallest score, and how many there are
   float best = -INFINITY, least = INFINITY;
   int some = 0;
   for (int i0 = tid; i0 < C; i0 += kBatch * THREADS) {
     float v[kBatch];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) v[b] = i0 + b * THREADS < C ? scores[i0 + b * THREADS] : -INFINITY;
+    for (int b = 0; b < kBatch; ++b) v[b] = i0 + b * THREADS < C ? score(i0 + b * THREADS) : -INFINITY;
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      if (kCached && i0 + b * THREADS < C) cache[i0 + b * THREADS] = v[b];
       if (v[b] > -INFINITY) {
         best = fmaxf(best, v[b]);
         least = fminf(least, v[b]);
@@ -280,7 +311,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       }
     }
   }
-  block.reduce(best, Most(), least, Least(), some, Add());  // and the barrier behind the cache
+  block.reduce(best, Most(), least, Least(), some, Add());
   if (some == 0 || !(T > 0.0)) {
     for (int d = tid; d < n; d += THREADS) {
       indices[d] = -1;
@@ -288,14 +319,17 @@ sample_rows_kernel(const __grid_constant__ Args A) {
     }
     return;
   }
-  const double inv_T = 1.0 / T, scale = ldexp(1.0, A.shift);
+  const double inv_T = 1.0 / T, per_bit = inv_T * 1.4426950408889634;
   // candidates are the scores from `first` on (false for NaN and -inf)
-  const float first = first_score(best, T, kLeast, 0.0, (double)best + kLeast * T);
+  const float first = (double)least - (double)best > -699.0 * T
+                          ? least
+                          : first_score(best, T, kLeast, 0.0, (double)best + kLeast * T);
 
   // The filters keep a prefix: scores above `cut`, and those equal to it up to index `cut_index`.
   float cut = -INFINITY;
   int32_t cut_index = -1;
   const auto inside = [&](float v, int i) { return v > cut || (v == cut && i <= cut_index); };
+  const double best_d = finite(best);
 
   const int64_t k = A.top_k.at(row);
   const double p = A.top_p.at(row);
@@ -318,17 +352,19 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   for (int masses = 0; masses < 2; ++masses) {
     if (masses ? !by_mass : !(by_count && k < some)) continue;
     double limit = (double)k;
-    float high = best, low = fmaxf(least, first);
+    float high = best, low = fmaxf(fmaxf(least, first), cut);
     if (masses) {  // below -(shift + 2) ln 2 a mass rounds to none
       const float none = best + (-0.6931472f * (A.shift + 2)) * (float)T;
-      low = fminf(fmaxf(fmaxf(low, cut), none), best);
+      low = fminf(fmaxf(low, none), best);
     }
-    const auto weight = [&](float v) { return masses ? mass_of(v, best, inv_T, scale) : 1ull; };
+    const auto weight = [&](float v) { return masses ? mass_of(v, best_d, per_bit, A.shift) : 1ull; };
     const auto enough = [&](unsigned long long sum) { return !((double)sum < limit); };
     unsigned long long above = 0;
     bool fresh = true;
     for (;;) {
-      const auto member = [&](float v, int i) { return v >= low && v <= high && inside(v, i); };
+      const auto member = [&](float v, int i) {  // low is at least the cut
+        return v >= low && v <= high && (v != cut || i <= cut_index);
+      };
       // the map falls with the score; in halves where a difference would overflow
       const float half = high - low < 3e38f ? 1.f : 0.5f;
       const float per = (kBins - 1) / (half * high - half * low);
@@ -339,23 +375,34 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       for (int i = tid; i < kBins; i += THREADS) sh.bins[0][i] = sh.bins[1][i] = 0;
       if (tid == 0) sh.members = 0;
       __syncthreads();
-      for (int i = tid; i < C; i += THREADS) {
-        const float v = score(i);
-        if (!member(v, i)) continue;
-        const int bin = bin_of(v);
-        if (masses) {
-          const unsigned long long w = weight(v);
-          if (w) {
-            const uint32_t lo = (uint32_t)w, old = atomicAdd(&sh.bins[0][bin], lo);
-            const uint32_t up = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
+      if (masses) {
+        for (int i0 = tid; i0 < C; i0 += kBatch * THREADS) {
+          unsigned long long w[kBatch];
+          float v[kBatch];
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int i = i0 + b * THREADS;
+            v[b] = i < C ? score(i) : -INFINITY;
+            w[b] = mass_here(fmaxf(v[b], low), best_d, per_bit, A.shift);
+            if (!member(v[b], i)) w[b] = 0;
+          }
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            if (w[b] == 0) continue;
+            const int bin = bin_of(v[b]);
+            const uint32_t lo = (uint32_t)w[b], old = atomicAdd(&sh.bins[0][bin], lo);
+            const uint32_t up = (uint32_t)(w[b] >> 32) + (old + lo < old ? 1u : 0u);
             if (up) atomicAdd(&sh.bins[1][bin], up);
           }
-        } else {  // lanes that all meet in one bin are added up first
-          const unsigned active = __activemask();
-          int same;
-          __match_all_sync(active, bin, &same);
-          if (!same) atomicAdd(&sh.bins[0][bin], 1u);
-          else if ((tid & 31) == __ffs(active) - 1) atomicAdd(&sh.bins[0][bin], (uint32_t)__popc(active));
+        }
+      } else {
+        for (int i0 = tid; i0 < C; i0 += kBatch * THREADS) {
+          float v[kBatch];
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) v[b] = i0 + b * THREADS < C ? score(i0 + b * THREADS) : -INFINITY;
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b)
+            if (member(v[b], i0 + b * THREADS)) atomicAdd(&sh.bins[0][bin_of(v[b])], 1u);
         }
       }
       __syncthreads();
@@ -396,7 +443,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
         }
         __syncthreads();
         if (tid < members) {
-#pragma unroll 1
+#pragma unroll 4
           for (int j = 0; j < members; ++j) {
             const float v = sh.ranked.score[j];
             rank += v > mine || (v == mine && sh.list[j] < index);
@@ -468,39 +515,42 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       by_share ? fmaxf(first, first_score(best, T, 0.0, least_share, (double)best + T * log(least_share))) : first;
   const auto kept = [&](float v, int i) { return v >= floor_score && inside(v, i); };
 
-  // The race in 32 bits: lower bounds.  a is off by a few 2^-24 of its size, the outer
-  // logarithm by 2^-21; with -4.7 < -log(-log u) < 16.7 for a uniform strictly between 0
-  // and 1 the size of either is at most |sum| + 17.
+  // The race in 32 bits: lower bounds.  -log u is a polynomial in 1 - u where u is near 1 (to
+  // 3e-6 of its size) and the hardware's logarithm elsewhere (2^-22 of at least 0.06); the
+  // outer logarithm is off by 2^-22 and what its argument is off by, a by a few 2^-24 of its size.  With
+  // -4.6 < -log(-log u) < 16.7 that is less than a quarter of the 1e-6 (|sum| + 40) taken off.
   const float inv_Tf = (float)inv_T;
   const auto lower = [&](float v, float u) {
-    const float g = (v == best ? 0.f : fmaxf(v - best, -3.4e38f) * inv_Tf) - __logf(-logf(u));
+    const float t = 1.f - u;
+    const float l = t < 0.0625f ? t * (1.f + t * (0.5f + t * (0.33333333f + t * 0.25f))) : -__logf(u);
+    const float g = (v == best ? 0.f : fmaxf(v - best, -3.4e38f) * inv_Tf) - __logf(l);
     return g - 1e-6f * (fabsf(g) + 40.f);
   };
+  constexpr float kLeastUniform = 1.17549435e-38f;  // subnormal ones are raced in 64 bits
   const bool filtered = by_count || by_mass || by_share;
-  const double per_bit = inv_T * 1.4426950408889634;
   double total = 0.0;
   float g_most = -INFINITY, g_least = INFINITY;
-  int open = 0, odd = 0;  // candidates in the race; uniforms of 0 and 1
+  int open = 0, odd = 0;  // candidates in the race; 1: a uniform of 0, 2: of 1 or subnormal
   __syncthreads();
   if (tid == 0) sh.members = 0;
   __syncthreads();
-  for (int i0 = tid; i0 < C; i0 += 2 * THREADS) {
-    float v[2], u[2];
-    bool in[2];
+  for (int i0 = tid; i0 < C; i0 += kBatch * THREADS) {
+    float v[kBatch], u[kBatch];
+    bool in[kBatch];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBatch; ++b) {
       const int i = i0 + b * THREADS;
       v[b] = i < C ? score(i) : -INFINITY;
       in[b] = kept(v[b], i);
       u[b] = in[b] ? uniforms[i] : 0.f;
     }
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBatch; ++b) {
       const int i = i0 + b * THREADS;
       float g = -INFINITY;
       if (in[b]) {
-        total += v[b] == best ? 1.0 : exp2_short(((double)v[b] - (double)best) * per_bit);
-        if (u[b] > 0.f && u[b] < 1.f) {
+        total += exp2_series<7>((finite(v[b]) - best_d) * per_bit, 0);
+        if (u[b] >= kLeastUniform && u[b] < 1.f) {
           g = lower(v[b], u[b]);
           g_most = fmaxf(g_most, g);
           g_least = fminf(g_least, g);
@@ -509,8 +559,8 @@ sample_rows_kernel(const __grid_constant__ Args A) {
             const int at = atomicAdd(&sh.members, 1);
             if (at < kFew) sh.list[at] = i;
           }
-        } else if (u[b] == 0.f || u[b] == 1.f) {
-          odd |= u[b] == 1.f ? 2 : 1;
+        } else if (u[b] >= 0.f && u[b] <= 1.f) {
+          odd |= u[b] > 0.f ? 2 : 1;
         }
       }
       if (kCached && i < C) cache[i] = g;
@@ -526,7 +576,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       const auto bound = [&](int i) {
         if (kCached) return cache[i];
         const float v = scores[i], u = uniforms[i];
-        return kept(v, i) && u > 0.f && u < 1.f ? lower(v, u) : -INFINITY;
+        return kept(v, i) && u >= kLeastUniform && u < 1.f ? lower(v, u) : -INFINITY;
       };
       float edge = g_least;  // at least n lower bounds reach it
       __syncthreads();
@@ -573,7 +623,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
           const unsigned long long mine = sh.race[tid];
           const int i = sh.list[tid];
           int rank = 0;
-#pragma unroll 2
+#pragma unroll 4
           for (int o = 0; o < members; ++o) {
             const unsigned long long other = sh.race[o];
             rank += other > mine || (other == mine && sh.list[o] < i);
@@ -623,7 +673,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       return;
     }
   }
-  // Uniforms of 0 or 1 among the draws, more equal race values than are
+  // Uniforms of 0, 1 or below the normal range among the draws, more equal race values than are
   // listed, or nobody in the race: one pass for each draw, over the row in memory.
   double last = INFINITY;
   int last_index = -1;
