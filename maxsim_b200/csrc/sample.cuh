@@ -178,7 +178,6 @@ struct Or {
 constexpr int kRaced = 2048;         // candidates of a row that are raced in 64 bits (a power of two)
 constexpr int kFew = 384;            // kept candidates that go to the 64-bit race without the 32-bit one
 constexpr int kMostCached = 40960;   // columns of a row in shared memory
-constexpr int kBatch = 4;            // elements of a thread whose loads are in flight together
 
 template <int THREADS>
 struct Shared {
@@ -261,6 +260,25 @@ struct Block {
   }
 };
 
+// Four consecutive elements of a row, `none` behind its end.
+struct Quad {
+  float v[4];
+};
+__device__ __forceinline__ Quad load_quad(const float* row, int q, int C, float none) {
+  Quad out;
+  if (4 * q + 3 < C && ((uintptr_t)row & 15) == 0) {
+    const float4 f = reinterpret_cast<const float4*>(row)[q];
+    out.v[0] = f.x; out.v[1] = f.y; out.v[2] = f.z; out.v[3] = f.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out.v[e] = 4 * q + e < C ? row[4 * q + e] : none;
+  }
+  return out;
+}
+__device__ __forceinline__ float most_of(const Quad& x) {  // NaN is none
+  return fmaxf(fmaxf(x.v[0], x.v[1]), fmaxf(x.v[2], x.v[3]));
+}
+
 template <int THREADS, bool kCached>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 sample_rows_kernel(const __grid_constant__ Args A) {
@@ -277,7 +295,14 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   float* const probabilities = A.probabilities + row * n;
   const double T = A.temperature.at(row);
 
+  const int quads = (C + 3) / 4;
   const auto score = [&](int i) { return kCached ? cache[i] : scores[i]; };
+  const auto score_quad = [&](int q) {
+    if (!kCached) return load_quad(scores, q, C, -INFINITY);
+    Quad out;
+    *reinterpret_cast<float4*>(&out) = reinterpret_cast<const float4*>(cache)[q];
+    return out;
+  };
 
   // The row comes into shared memory with everything in flight at once; its uniforms, needed
   // several passes later, are asked into L2 meanwhile.
@@ -289,6 +314,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       for (int i = tid; i < C; i += THREADS) copy_async<4>(cache + i, scores + i);
     }
     copies_commit();
+    if (C + tid < 4 * quads) cache[C + tid] = -INFINITY;
   }
   for (int i = 32 * tid; i < C; i += 32 * THREADS) asm volatile("prefetch.global.L2 [%0];" ::"l"(uniforms + i));
   if (kCached) {
@@ -298,17 +324,14 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   // the largest and the smallest score, and how many there are
   float best = -INFINITY, least = INFINITY;
   int some = 0;
-  for (int i0 = tid; i0 < C; i0 += kBatch * THREADS) {
-    float v[kBatch];
+  for (int q = tid; q < quads; q += THREADS) {
+    const Quad x = score_quad(q);
+    best = fmaxf(best, most_of(x));
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) v[b] = i0 + b * THREADS < C ? score(i0 + b * THREADS) : -INFINITY;
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      if (v[b] > -INFINITY) {
-        best = fmaxf(best, v[b]);
-        least = fminf(least, v[b]);
-        ++some;
-      }
+    for (int e = 0; e < 4; ++e) {
+      const bool there = x.v[e] > -INFINITY;
+      least = fminf(least, there ? x.v[e] : INFINITY);
+      some += there;
     }
   }
   block.reduce(best, Most(), least, Least(), some, Add());
@@ -376,33 +399,31 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       if (tid == 0) sh.members = 0;
       __syncthreads();
       if (masses) {
-        for (int i0 = tid; i0 < C; i0 += kBatch * THREADS) {
-          unsigned long long w[kBatch];
-          float v[kBatch];
+        for (int q = tid; q < quads; q += THREADS) {
+          const Quad x = score_quad(q);
+          if (!(most_of(x) >= low)) continue;
+          unsigned long long w[4];
 #pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
-            const int i = i0 + b * THREADS;
-            v[b] = i < C ? score(i) : -INFINITY;
-            w[b] = mass_here(fmaxf(v[b], low), best_d, per_bit, A.shift);
-            if (!member(v[b], i)) w[b] = 0;
+          for (int e = 0; e < 4; ++e) {
+            w[e] = mass_here(fmaxf(x.v[e], low), best_d, per_bit, A.shift);
+            if (!member(x.v[e], 4 * q + e)) w[e] = 0;
           }
 #pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
-            if (w[b] == 0) continue;
-            const int bin = bin_of(v[b]);
-            const uint32_t lo = (uint32_t)w[b], old = atomicAdd(&sh.bins[0][bin], lo);
-            const uint32_t up = (uint32_t)(w[b] >> 32) + (old + lo < old ? 1u : 0u);
+          for (int e = 0; e < 4; ++e) {
+            if (w[e] == 0) continue;
+            const int bin = bin_of(x.v[e]);
+            const uint32_t lo = (uint32_t)w[e], old = atomicAdd(&sh.bins[0][bin], lo);
+            const uint32_t up = (uint32_t)(w[e] >> 32) + (old + lo < old ? 1u : 0u);
             if (up) atomicAdd(&sh.bins[1][bin], up);
           }
         }
       } else {
-        for (int i0 = tid; i0 < C; i0 += kBatch * THREADS) {
-          float v[kBatch];
+        for (int q = tid; q < quads; q += THREADS) {
+          const Quad x = score_quad(q);
+          if (!(most_of(x) >= low)) continue;
 #pragma unroll
-          for (int b = 0; b < kBatch; ++b) v[b] = i0 + b * THREADS < C ? score(i0 + b * THREADS) : -INFINITY;
-#pragma unroll
-          for (int b = 0; b < kBatch; ++b)
-            if (member(v[b], i0 + b * THREADS)) atomicAdd(&sh.bins[0][bin_of(v[b])], 1u);
+          for (int e = 0; e < 4; ++e)
+            if (member(x.v[e], 4 * q + e)) atomicAdd(&sh.bins[0][bin_of(x.v[e])], 1u);
         }
       }
       __syncthreads();
@@ -422,13 +443,24 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       const int bin = sh.found_bin;
       above = sh.found_above;
       float most = -INFINITY, fewest = INFINITY;
-      for (int i = tid; i < C; i += THREADS) {
-        const float v = score(i);
-        if (!member(v, i) || bin_of(v) != bin) continue;
-        most = fmaxf(most, v);
-        fewest = fminf(fewest, v);
-        const int at = atomicAdd(&sh.members, 1);
-        if (at < kListed) sh.list[at] = i;
+      // nothing of the bin lies below this: its lower end, a hundredth of its width and the rounding beyond
+      const float lowest = low == high || !(per < 3e38f)
+                               ? low
+                               : fmaxf(low, (half * high - (bin + 1.01f) / per) / half -
+                                                4e-7f * fmaxf(fabsf(high), fabsf(low)));
+      for (int q = tid; q < quads; q += THREADS) {
+        const Quad x = score_quad(q);
+        if (!(most_of(x) >= lowest)) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = x.v[e];
+          const int i = 4 * q + e;
+          if (!(v >= lowest) || !member(v, i) || bin_of(v) != bin) continue;
+          most = fmaxf(most, v);
+          fewest = fminf(fewest, v);
+          const int at = atomicAdd(&sh.members, 1);
+          if (at < kListed) sh.list[at] = i;
+        }
       }
       block.reduce(most, Most(), fewest, Least());
       const int members = sh.members;
@@ -443,11 +475,15 @@ sample_rows_kernel(const __grid_constant__ Args A) {
         }
         __syncthreads();
         if (tid < members) {
-#pragma unroll 4
+          int equal = 0;
+#pragma unroll 8
           for (int j = 0; j < members; ++j) {
             const float v = sh.ranked.score[j];
-            rank += v > mine || (v == mine && sh.list[j] < index);
+            rank += v > mine;
+            equal += v == mine;
           }
+          if (equal > 1)
+            for (int j = 0; j < members; ++j) rank += sh.ranked.score[j] == mine && sh.list[j] < index;
         }
         __syncthreads();
         if (tid < members) {
@@ -534,37 +570,33 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   __syncthreads();
   if (tid == 0) sh.members = 0;
   __syncthreads();
-  for (int i0 = tid; i0 < C; i0 += kBatch * THREADS) {
-    float v[kBatch], u[kBatch];
-    bool in[kBatch];
+  const float lowest_kept = fmaxf(floor_score, cut);
+  for (int q = tid; q < quads; q += THREADS) {
+    const Quad x = score_quad(q);
+    Quad g;
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int i = i0 + b * THREADS;
-      v[b] = i < C ? score(i) : -INFINITY;
-      in[b] = kept(v[b], i);
-      u[b] = in[b] ? uniforms[i] : 0.f;
-    }
+    for (int e = 0; e < 4; ++e) g.v[e] = -INFINITY;
+    if (most_of(x) >= lowest_kept) {
+      const Quad u = load_quad(uniforms, q, C, -1.f);
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int i = i0 + b * THREADS;
-      float g = -INFINITY;
-      if (in[b]) {
-        total += exp2_series<7>((finite(v[b]) - best_d) * per_bit, 0);
-        if (u[b] >= kLeastUniform && u[b] < 1.f) {
-          g = lower(v[b], u[b]);
-          g_most = fmaxf(g_most, g);
-          g_least = fminf(g_least, g);
+      for (int e = 0; e < 4; ++e) {
+        if (!kept(x.v[e], 4 * q + e)) continue;
+        total += exp2_series<7>((finite(x.v[e]) - best_d) * per_bit, 0);
+        if (u.v[e] >= kLeastUniform && u.v[e] < 1.f) {
+          g.v[e] = lower(x.v[e], u.v[e]);
+          g_most = fmaxf(g_most, g.v[e]);
+          g_least = fminf(g_least, g.v[e]);
           ++open;
           if (filtered) {
             const int at = atomicAdd(&sh.members, 1);
-            if (at < kFew) sh.list[at] = i;
+            if (at < kFew) sh.list[at] = 4 * q + e;
           }
-        } else if (u[b] >= 0.f && u[b] <= 1.f) {
-          odd |= u[b] > 0.f ? 2 : 1;
+        } else if (u.v[e] >= 0.f && u.v[e] <= 1.f) {
+          odd |= u.v[e] > 0.f ? 2 : 1;
         }
       }
-      if (kCached && i < C) cache[i] = g;
     }
+    if (kCached) reinterpret_cast<float4*>(cache)[q] = *reinterpret_cast<const float4*>(&g);
   }
   block.reduce(total, Add(), g_most, Most(), g_least, Least(), open, Add(), odd, Or());
 
@@ -573,10 +605,18 @@ sample_rows_kernel(const __grid_constant__ Args A) {
     int members = open;
     if (!filtered || open > kFew) {
       const float per = g_most > g_least ? (kBins - 1) / (g_most - g_least) : 0.f;
-      const auto bound = [&](int i) {
-        if (kCached) return cache[i];
-        const float v = scores[i], u = uniforms[i];
-        return kept(v, i) && u >= kLeastUniform && u < 1.f ? lower(v, u) : -INFINITY;
+      const auto bounds = [&](int q) {
+        Quad g = score_quad(q);
+        if (kCached || !(most_of(g) >= lowest_kept)) {
+          if (!kCached)
+            for (int e = 0; e < 4; ++e) g.v[e] = -INFINITY;
+          return g;
+        }
+        const Quad u = load_quad(uniforms, q, C, -1.f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          g.v[e] = kept(g.v[e], 4 * q + e) && u.v[e] >= kLeastUniform && u.v[e] < 1.f ? lower(g.v[e], u.v[e]) : -INFINITY;
+        return g;
       };
       float edge = g_least;  // at least n lower bounds reach it
       __syncthreads();
@@ -584,9 +624,12 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       if (open > n) {
         for (int i = tid; i < kBins; i += THREADS) sh.bins[0][i] = 0;
         __syncthreads();
-        for (int i = tid; i < C; i += THREADS) {
-          const float g = bound(i);
-          if (g > -INFINITY) atomicAdd(&sh.bins[0][min((int)((g_most - g) * per), kBins - 1)], 1u);
+        for (int q = tid; q < quads; q += THREADS) {
+          const Quad g = bounds(q);
+          if (!(most_of(g) >= g_least)) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (g.v[e] >= g_least) atomicAdd(&sh.bins[0][min((int)((g_most - g.v[e]) * per), kBins - 1)], 1u);
         }
         __syncthreads();
         const unsigned long long c0 = sh.bins[0][2 * tid], c1 = sh.bins[0][2 * tid + 1];
@@ -600,10 +643,15 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       }
       edge -= 2.1e-6f * (fabsf(edge) + 41.f);  // what an upper bound may lie above its lower one
       __syncthreads();
-      for (int i = tid; i < C; i += THREADS) {
-        if (bound(i) < edge) continue;
-        const int at = atomicAdd(&sh.members, 1);
-        if (at < kRaced) sh.list[at] = i;
+      for (int q = tid; q < quads; q += THREADS) {
+        const Quad g = bounds(q);
+        if (!(most_of(g) >= edge)) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (!(g.v[e] >= edge)) continue;
+          const int at = atomicAdd(&sh.members, 1);
+          if (at < kRaced) sh.list[at] = 4 * q + e;
+        }
       }
       __syncthreads();
       members = sh.members;
@@ -622,12 +670,15 @@ sample_rows_kernel(const __grid_constant__ Args A) {
         if (tid < members) {
           const unsigned long long mine = sh.race[tid];
           const int i = sh.list[tid];
-          int rank = 0;
-#pragma unroll 4
+          int rank = 0, equal = 0;
+#pragma unroll 8
           for (int o = 0; o < members; ++o) {
             const unsigned long long other = sh.race[o];
-            rank += other > mine || (other == mine && sh.list[o] < i);
+            rank += other > mine;
+            equal += other == mine;
           }
+          if (equal > 1)
+            for (int o = 0; o < members; ++o) rank += sh.race[o] == mine && sh.list[o] < i;
           if (rank < n) {
             indices[rank] = i;
             probabilities[rank] = share_of(scores[i], best, T, total);
