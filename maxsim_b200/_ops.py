@@ -16,6 +16,7 @@ library, is an error.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import types
 import weakref
@@ -186,16 +187,17 @@ def contrastive_ce(scores: torch.Tensor, targets: torch.Tensor, temperature: flo
     return loss_rows, dscore
 
 
-def offsets_from_lengths(lengths: torch.Tensor, L_max: int):
+def offsets_from_lengths(lengths: torch.Tensor, L_max: int, want_total: bool = True):
     """``lengths [N]`` (CUDA, integer) -> ``(offsets [N+1] int32, total [1] int64)``,
-    both on the device; lengths are clamped to ``[0, L_max]``."""
+    both on the device; lengths are clamped to ``[0, L_max]``.  The total is None
+    unless wanted."""
     dev = _require_cuda(lengths)
     ln = _i32(lengths.reshape(-1))
-    offsets = torch.empty((ln.shape[0] + 1,), dtype=torch.int32, device=dev)
-    total = torch.empty((1,), dtype=torch.int64, device=dev)
+    offsets = ln.new_empty((ln.shape[0] + 1,))
+    total = torch.empty((1,), dtype=torch.int64, device=dev) if want_total else None
     with _on_device(dev):
         rc = load_library().maxsim_b200_offsets_from_lengths(
-            _ptr(ln), ln.shape[0], int(L_max), offsets.data_ptr(), total.data_ptr(), _stream_ptr())
+            _ptr(ln), ln.shape[0], int(L_max), offsets.data_ptr(), _opt(total), _stream_ptr())
     _check(rc, "maxsim_b200_offsets_from_lengths")
     return offsets, total
 
@@ -284,19 +286,17 @@ def sample_rows(scores: torch.Tensor, uniforms: torch.Tensor, n: int, temperatur
     Each of the four parameters is a number or a ``[rows]`` tensor (fp32, int32
     for ``top_k``) on the same device; ``top_k`` 0, ``top_p`` 1 and ``min_p`` 0
     filter nothing."""
-    params = []
-    for value in (temperature, top_k, top_p, min_p):
-        params += [0, value] if isinstance(value, torch.Tensor) else [value, None]
-    dev = _require_cuda(scores, uniforms, *(t for t in params[1::2] if t is not None))
+    dev = _require_cuda(scores, uniforms,
+                        *[t for t in (temperature, top_k, top_p, min_p) if isinstance(t, torch.Tensor)])
+    pair = lambda t: (0, _ptr(t)) if isinstance(t, torch.Tensor) else (t, 0)  # noqa: E731
     rows, cols = scores.shape
-    indices = torch.empty((rows, int(n)), dtype=torch.int64, device=dev)
-    probabilities = torch.empty((rows, int(n)), dtype=torch.float32, device=dev)
-    for i in (1, 3, 5, 7):
-        params[i] = 0 if params[i] is None else _ptr(params[i])
+    indices = scores.new_empty((rows, n), dtype=torch.int64)
+    probabilities = scores.new_empty((rows, n))
     with _on_device(dev):
         rc = load_library().maxsim_b200_sample_rows(
-            _ptr(scores), scores.stride(0), _ptr(uniforms), uniforms.stride(0), rows, cols, int(n),
-            *params, _ptr(indices), _ptr(probabilities), _stream_ptr())
+            _ptr(scores), scores.stride(0), _ptr(uniforms), uniforms.stride(0), rows, cols, n,
+            *pair(temperature), *pair(top_k), *pair(top_p), *pair(min_p),
+            _ptr(indices), _ptr(probabilities), _stream_ptr())
     _check(rc, "maxsim_b200_sample_rows")
     return indices, probabilities
 
@@ -309,41 +309,50 @@ def norm_rows(kind: int, tokens: torch.Tensor, strides, shape, offsets, packed_r
     """Normalise the rows of ``tokens``: ``shape`` is ``(n_segments, L_max, dim)``
     and ``strides`` the element strides of its first two dimensions (the last
     is contiguous).  With ``offsets [n_segments + 1]`` int32 the rows that count
-    are written back to back.  Returns ``(out [packed_rows, dim], mean, rstd)``;
-    the statistics are None unless asked for (layer norm only)."""
-    dev = _require_cuda(*(t for t in (tokens, offsets, weight, bias) if t is not None))
+    are written back to back.  Returns ``(out [packed_rows, dim], stats)``; the
+    statistics ``[2, packed_rows]`` fp32 (means, then reciprocal standard
+    deviations) are None unless asked for (layer norm only)."""
+    dev = tokens.device
     n, L, dim = shape
-    out = torch.empty((packed_rows, dim), dtype=tokens.dtype, device=dev)
-    mean = rstd = None
-    if want_stats:
-        mean, rstd = torch.empty((2, packed_rows), dtype=torch.float32, device=dev)
+    out = tokens.new_empty((packed_rows, dim))
+    stats = tokens.new_empty((2, packed_rows), dtype=torch.float32) if want_stats else None
+    at = _ptr(stats) if want_stats else 0
     with _on_device(dev):
         rc = load_library().maxsim_b200_norm_rows(
             kind, _ptr(tokens), strides[0], strides[1], offsets.data_ptr() if offsets is not None else 0,
-            _opt(weight), _opt(bias), _ptr(out), _opt(mean), _opt(rstd), n, L, dim, packed_rows, eps,
+            _opt(weight), _opt(bias), _ptr(out), at, at + 4 * packed_rows if at else 0, n, L, dim, packed_rows, eps,
             _code(tokens), _code(weight) if weight is not None else 0, _stream_ptr())
     _check(rc, "maxsim_b200_norm_rows")
-    return out, mean, rstd
+    return out, stats
 
 
-def norm_rows_backward(kind: int, grad: torch.Tensor, tokens: torch.Tensor, strides, shape, offsets, weight,
-                       mean, rstd, eps: float, want_tokens: bool, want_weight: bool, want_bias: bool):
+@functools.lru_cache(maxsize=256)
+def _norm_workspace(device_index, n: int, L: int, dim: int) -> int:
+    """Bytes of workspace on the current device, which has the given index."""
+    return load_library().maxsim_b200_norm_rows_workspace(n, L, dim)
+
+
+def norm_rows_backward(kind: int, grad: torch.Tensor, tokens: torch.Tensor, strides, shape, offsets,
+                       packed_rows: int, weight, stats, eps: float, want_tokens: bool, want_weight: bool,
+                       want_bias: bool):
     """The gradients of :func:`norm_rows` that are wanted, else None:
-    ``(grad_tokens [n_segments, L_max, dim], grad_weight [dim], grad_bias [dim])``."""
-    dev = _require_cuda(*(t for t in (tokens, grad, offsets, weight, mean, rstd) if t is not None))
+    ``(grad_tokens [n_segments * L_max * dim], grad_weight [dim], grad_bias
+    [dim])`` from the contiguous ``grad [packed_rows, dim]``."""
+    dev = tokens.device
     n, L, dim = shape
-    lib = load_library()
-    dx = torch.empty(shape, dtype=tokens.dtype, device=dev) if want_tokens else None
-    dw = torch.empty((dim,), dtype=weight.dtype, device=dev) if want_weight else None
-    db = torch.empty((dim,), dtype=weight.dtype, device=dev) if want_bias else None
+    dx = tokens.new_empty((n * L * dim,)) if want_tokens else None
+    dw = torch.empty_like(weight) if want_weight else None
+    db = torch.empty_like(weight) if want_bias else None
+    at = _opt(stats)
     with _on_device(dev):
-        work = None
+        work, size = None, 0
         if want_weight or want_bias:
-            work = torch.empty((lib.maxsim_b200_norm_rows_workspace(n, L, dim),), dtype=torch.uint8, device=dev)
-        rc = lib.maxsim_b200_norm_rows_backward(
+            size = _norm_workspace(dev.index, n, L, dim)
+            work = tokens.new_empty((size,), dtype=torch.uint8)
+        rc = load_library().maxsim_b200_norm_rows_backward(
             kind, _ptr(grad), _ptr(tokens), strides[0], strides[1],
-            offsets.data_ptr() if offsets is not None else 0, _opt(weight), _opt(mean), _opt(rstd), _opt(dx),
-            _opt(dw), _opt(db), _opt(work), work.numel() if work is not None else 0, n, L, dim, grad.shape[0], eps,
+            offsets.data_ptr() if offsets is not None else 0, _opt(weight), at, at + 4 * packed_rows if at else 0,
+            _opt(dx), _opt(dw), _opt(db), _opt(work), size, n, L, dim, packed_rows, eps,
             _code(tokens), _code(weight) if weight is not None else 0, _stream_ptr())
     _check(rc, "maxsim_b200_norm_rows_backward")
     return dx, dw, db

@@ -205,7 +205,7 @@ int launch(int kind, int dtype, const Call& call) {
 
 template <typename W>
 int launch_sum(const Backward& call, void* grad_weight, void* grad_bias) {
-  norm::grad_weight_sum_kernel<W><<<dim3((unsigned)ceil_div(call.t.dim, 32), 2), norm::kThreads, 0, call.st>>>(
+  norm::grad_weight_sum_kernel<W><<<dim3((unsigned)ceil_div(call.t.dim, 32), 2), norm::kSumThreads, 0, call.st>>>(
       call.partial, call.slabs, call.t.dim, (W*)grad_weight, (W*)grad_bias);
   return launch_check("norm grad_weight_sum_kernel");
 }

@@ -737,29 +737,28 @@ backward_rows_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, c
   }
 }
 
-// Adds the rows of partial [2][slabs][dim] in order: a CTA takes 32 columns of
-// one of the two halves, its 8 warps every eighth row.
+// Adds the rows of partial [2][slabs][dim] in a fixed order: a CTA takes 32 columns of
+// one of the two halves, its 32 warps every 32nd row.
+constexpr int kSumThreads = 1024;
 template <typename W>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kSumThreads)
 grad_weight_sum_kernel(const float* __restrict__ partial, int slabs, int dim, W* __restrict__ grad_weight,
                        W* __restrict__ grad_bias) {
-  __shared__ float acc[kThreads / 32][32];
+  constexpr int kWarps = kSumThreads / 32;
+  __shared__ float acc[kWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   W* to = blockIdx.y ? grad_bias : grad_weight;
   if (!to) return;
   const float* from = partial + (int64_t)blockIdx.y * slabs * dim;
   float sum = 0.f;
   if (c < dim) {
-#pragma unroll 4
-    for (int s = warp; s < slabs; s += kThreads / 32) sum += from[(int64_t)s * dim + c];
+#pragma unroll 8
+    for (int s = warp; s < slabs; s += kWarps) sum += from[(int64_t)s * dim + c];
   }
   acc[warp][lane] = sum;
   __syncthreads();
-  if (warp == 0 && c < dim) {
-#pragma unroll
-    for (int w = 1; w < kThreads / 32; ++w) sum += acc[w][lane];
-    to[c] = narrow<W>(sum);
-  }
+  sum = warp_sum(acc[lane][warp]);  // warp w adds up column w
+  if (lane == 0 && blockIdx.x * 32 + warp < dim) to[blockIdx.x * 32 + warp] = narrow<W>(sum);
 }
 
 // ---------------------------------------------------------------------------

@@ -84,7 +84,7 @@ def packed_offsets(padded: torch.Tensor, lengths: torch.Tensor, total_tokens: Op
             raise ValueError("packed token count must fit int32 offsets")
         offsets = host.to(torch.int32).to(padded.device, non_blocking=True)
     else:
-        offsets, total_dev = _ops.offsets_from_lengths(lengths, L_max)
+        offsets, total_dev = _ops.offsets_from_lengths(lengths, L_max, total_tokens is None)
         if total_tokens is None:
             total = int(total_dev.item())
             if total >= 2 ** 31:
@@ -203,7 +203,8 @@ def sample_candidates(scores: torch.Tensor, uniforms: torch.Tensor, n: int, *, t
     if uniforms.dtype != torch.float32:
         raise TypeError(f"uniforms must be float32; got {uniforms.dtype}")
     B, C = scores.shape
-    if not 0 <= index(n) <= min(C, 1024):
+    n = index(n)
+    if not 0 <= n <= min(C, 1024):
         raise ValueError(f"n must be in [0, min(C={C}, 1024)]; got {n}")
     if C > 2 ** 20:
         raise ValueError(f"scores may have at most 2^20 candidates per row; got {C}")
@@ -216,9 +217,13 @@ def sample_candidates(scores: torch.Tensor, uniforms: torch.Tensor, n: int, *, t
               1.0 if top_p is None else _per_row("top_p", top_p, B, torch.float32, scores.device, 0, 1),
               0.0 if min_p is None or (not isinstance(min_p, torch.Tensor) and min_p == 0)
               else _per_row("min_p", min_p, B, torch.float32, scores.device, 0, 1)]
-    s = scores.detach().to(torch.float32)
-    s, u = (t if t.stride(1) == 1 or C == 1 else t.contiguous() for t in (s, uniforms.detach()))
-    return _ops.sample_rows(s, u, int(n), *params)
+    if scores.dtype != torch.float32:
+        scores = scores.detach().to(torch.float32)
+    if C > 1 and scores.stride(1) != 1:
+        scores = scores.contiguous()
+    if C > 1 and uniforms.stride(1) != 1:
+        uniforms = uniforms.contiguous()
+    return _ops.sample_rows(scores, uniforms, n, *params)
 
 
 _STAGING = {}

@@ -44,40 +44,58 @@ def _two_strides(t: torch.Tensor):
     return t, (1, t.numel() // dim if dim else 0), (0, dim)
 
 
+def _forward(kind, tokens, weight, bias, offsets, total, eps, want_stats):
+    """``offsets`` None: rows in, rows out.  Returns the result and what the
+    backward pass needs."""
+    if offsets is None:
+        src, (n, L), strides = _two_strides(tokens)
+        total = n * L
+    else:
+        src = tokens if tokens.stride(2) == 1 else tokens.contiguous()
+        n, L = src.shape[:2]
+        strides = (src.stride(0), src.stride(1))
+    call = (strides, (n, L, tokens.shape[-1]), offsets, total)
+    w = weight.contiguous() if weight is not None else None
+    b = bias.contiguous() if bias is not None else None
+    out, stats = _ops.norm_rows(kind, src, *call, w, b, eps, want_stats)
+    return out if offsets is not None else out.view(tokens.shape), src, w, stats, call
+
+
 class _NormFn(torch.autograd.Function):
-    """``offsets`` None: rows in, rows out.  The statistics of a layer norm are
-    saved for the backward pass; a unit row's length is taken again from the row."""
+    """The statistics of a layer norm are saved for the backward pass; a unit
+    row's length is taken again from the row."""
 
     @staticmethod
     def forward(ctx, kind, tokens, weight, bias, offsets, total, eps):
-        if offsets is None:
-            src, (n, L), strides = _two_strides(tokens)
-            total = n * L
-        else:
-            src = tokens if tokens.dim() == 3 and tokens.stride(2) == 1 else tokens.contiguous()
-            n, L = src.shape[:2]
-            strides = (src.stride(0), src.stride(1))
-        shape = (n, L, tokens.shape[-1])
-        train = any(ctx.needs_input_grad)
-        w = weight.contiguous() if weight is not None else None
-        out, mean, rstd = _ops.norm_rows(kind, src, strides, shape, offsets, total, w,
-                                         bias.contiguous() if bias is not None else None, eps,
-                                         train and kind == _ops.NORM_LAYER)
-        if train:
-            ctx.save_for_backward(src, w, offsets, mean, rstd)
-            ctx.call = (kind, strides, shape, eps, tokens.shape)
-        return out if offsets is not None else out.view(tokens.shape)
+        out, src, w, stats, call = _forward(kind, tokens, weight, bias, offsets, total, eps, kind == _ops.NORM_LAYER)
+        ctx.save_for_backward(src, w, stats, offsets)
+        ctx.call = (kind, call[0], call[1], call[3], eps, tokens.shape)
+        return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        src, w, offsets, mean, rstd = ctx.saved_tensors
-        kind, strides, shape, eps, token_shape = ctx.call
-        g = grad.reshape(-1, shape[2]).contiguous()
-        _, want_tokens, want_weight, want_bias = ctx.needs_input_grad[:4]
-        dx, dw, db = _ops.norm_rows_backward(kind, g, src, strides, shape, offsets, w, mean, rstd, eps,
-                                             want_tokens, want_weight, want_bias)
-        return None, dx.view(token_shape) if dx is not None else None, dw, db, None, None, None
+        if torch.is_grad_enabled():  # create_graph: what comes out cannot be differentiated again
+            return _backward_once(ctx, grad)
+        return _backward(ctx, grad)
+
+
+def _backward(ctx, grad):
+    src, w, stats, offsets = ctx.saved_tensors
+    kind, strides, shape, total, eps, token_shape = ctx.call
+    needs = ctx.needs_input_grad
+    dx, dw, db = _ops.norm_rows_backward(kind, grad.contiguous(), src, strides, shape, offsets, total, w, stats, eps,
+                                         needs[1], needs[2], needs[3])
+    return None, dx.view(token_shape) if dx is not None else None, dw, db, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
+
+
+def _apply(kind, tokens, weight, bias, offsets, total, eps):
+    if torch.is_grad_enabled() and (tokens.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _NormFn.apply(kind, tokens, weight, bias, offsets, total, eps)
+    return _forward(kind, tokens, weight, bias, offsets, total, eps, False)[0]
 
 
 def _check(name: str, tokens, weight, bias, eps) -> None:
@@ -102,8 +120,8 @@ def _check(name: str, tokens, weight, bias, eps) -> None:
         raise ValueError(f"eps must be at least 1e-30 and finite; got {eps}")
     if tokens.device.type != "cuda":
         raise RuntimeError(f"{name} must be a CUDA tensor (maxsim_b200 has no CPU path); got device {tokens.device}")
-    _v.require_same_device({n: t for n, t in ((name, tokens), ("weight", weight), ("bias", bias))
-                            if t is not None})
+    if weight is not None:
+        _v.require_same_device({name: tokens, "weight": weight, "bias": weight if bias is None else bias})
     if tokens.numel() // dim > 2 ** 31 - 4096:
         raise ValueError(f"{name} may have at most 2^31 - 4096 rows; got shape {tuple(tokens.shape)}")
 
@@ -113,7 +131,7 @@ def _packed(kind, padded, lengths, weight, bias, eps, total_tokens):
         raise ValueError(f"padded must be 3-D [N, L_max, D]; got shape {tuple(padded.shape)}")
     _check("padded", padded, weight, bias, eps)
     offsets, total = packed_offsets(padded, lengths, total_tokens)
-    return _NormFn.apply(kind, padded, weight, bias, offsets, total, float(eps)), offsets
+    return _apply(kind, padded, weight, bias, offsets, total, float(eps)), offsets
 
 
 @_eager
@@ -128,7 +146,7 @@ def layer_norm(tokens: torch.Tensor, weight: Optional[torch.Tensor] = None,
     their type.  Raises ``ValueError`` / ``TypeError`` for shapes and types
     outside this, ``RuntimeError`` for tensors that are not on one CUDA device."""
     _check("tokens", tokens, weight, bias, eps)
-    return _NormFn.apply(_ops.NORM_LAYER, tokens, weight, bias, None, 0, float(eps))
+    return _apply(_ops.NORM_LAYER, tokens, weight, bias, None, 0, float(eps))
 
 
 @_eager
@@ -150,7 +168,7 @@ def unit_norm(tokens: torch.Tensor, *, eps: float = 1e-12) -> torch.Tensor:
     defined on.  Differentiable; a row no longer than ``eps`` is scaled by a
     constant and has the gradient of that."""
     _check("tokens", tokens, None, None, eps)
-    return _NormFn.apply(_ops.NORM_UNIT, tokens, None, None, None, 0, float(eps))
+    return _apply(_ops.NORM_UNIT, tokens, None, None, None, 0, float(eps))
 
 
 @_eager
