@@ -55,7 +55,7 @@ struct Forward {
 
   template <typename T, int KIND, int E, int TEAM, int V>
   int rows() const {
-    constexpr int threads = norm::kCtaThreads<TEAM>, per_sm = norm::kForwardThreads<E, V>;
+    constexpr int threads = norm::kCtaThreads<TEAM>, per_sm = norm::kForwardThreads<E, TEAM, V>;
     constexpr int ring = norm::kRingBytes<T, E, TEAM, V, 1, per_sm>;
     auto kern = norm::forward_rows_kernel<T, KIND, E, TEAM, V>;
     static std::atomic<unsigned char> configured[kMaxDevices];
@@ -96,7 +96,7 @@ struct Backward {
 
   template <typename T, int KIND, int E, int TEAM, int V>
   int rows() const {
-    constexpr int threads = norm::kCtaThreads<TEAM>, per_sm = norm::kBackwardThreads<KIND, E, V>;
+    constexpr int threads = norm::kCtaThreads<TEAM>, per_sm = norm::kBackwardThreads<KIND, E, TEAM, V>;
     constexpr int fixed = norm::kBackwardBytes<T, KIND, E, TEAM, V>;
     auto kern = norm::backward_rows_kernel<T, KIND, E, TEAM, V>;
     static std::atomic<unsigned char> configured[kMaxDevices];
@@ -140,6 +140,10 @@ int by_width(const Call& call) {
   constexpr bool sums = Call::kSums && KIND == norm::kLayer;
   const int packs = (call.t.dim + E - 1) / E;
   if constexpr (E == 8) {
+    if constexpr (KIND == norm::kUnit) {
+      if (packs <= 2) return call.template rows<T, KIND, E, 2, 1>();
+      if (packs <= 4) return call.template rows<T, KIND, E, 4, 1>();
+    }
     if (packs <= 8) return call.template rows<T, KIND, E, 8, 1>();
     if (packs <= 16) return call.template rows<T, KIND, E, 8, 2>();
     if (packs <= 32) return call.template rows<T, KIND, E, 16, 2>();
@@ -165,13 +169,24 @@ int by_width(const Call& call) {
     if (packs <= 512) return call.template rows<T, KIND, E, norm::kWide, 4>();
     if (packs <= 1024) return call.template rows<T, KIND, E, norm::kWide, 8>();
   } else if constexpr (E == 2) {
-    if (packs <= 64) return call.template rows<T, KIND, E, 32, 2>();
+    if (packs <= 16) return call.template rows<T, KIND, E, 8, 2>();
+    if (packs <= 32) return call.template rows<T, KIND, E, 16, 2>();
+    if (packs <= 64) return call.template rows<T, KIND, E, 16, 4>();
+    if (packs <= 128) return call.template rows<T, KIND, E, 32, 4>();
     if (packs <= 192) return call.template rows<T, KIND, E, 32, 6>();
     if (packs <= 512) return call.template rows<T, KIND, E, 32, 16>();
+    if (packs <= 768) return call.template rows<T, KIND, E, norm::kWide, 6>();
     if (packs <= 2048) return call.template rows<T, KIND, E, norm::kWide, 16>();
   } else {
+    if (packs <= 32) return call.template rows<T, KIND, E, 32, 1>();
+    if (packs <= 64) return call.template rows<T, KIND, E, 32, 2>();
+    if (packs <= 96) return call.template rows<T, KIND, E, 32, 3>();
     if (packs <= 128) return call.template rows<T, KIND, E, 32, 4>();
+    if (packs <= 256) return call.template rows<T, KIND, E, 32, 8>();
     if (packs <= 384) return call.template rows<T, KIND, E, 32, 12>();
+    if constexpr (sums && sizeof(T) == 4) {
+      if (packs <= 1024) return call.template rows<T, KIND, E, norm::kWide, 8>();
+    }
     if (packs <= 1024) return call.template rows<T, KIND, E, 32, 32>();
     if (packs <= 4096) return call.template rows<T, KIND, E, norm::kWide, 32>();
   }

@@ -52,6 +52,10 @@ struct Rows {
   int32_t dim;
 
   __device__ __forceinline__ int32_t start(int32_t n) const { return offsets ? offsets[n] : n * L_max; }
+  // Where the last token row starts.
+  __device__ __forceinline__ int64_t last() const {
+    return (n_segments - 1) * segment_stride + (L_max - 1) * row_stride;
+  }
   // Packed rows that belong to a segment.
   __device__ __forceinline__ int32_t used() const { return min(rows, start(n_segments)); }
 };
@@ -242,31 +246,47 @@ __device__ __forceinline__ UnitScale unit_scale(float ss, float top, float eps) 
 // HBM-bound: what counts is bytes in flight.  Every thread copies its own packs of the
 // next rows into a ring in shared memory (cp.async) and reads back nothing but
 // what it copied itself, so the ring needs no barrier; the reductions and the store of a row run
-// under the loads of the next kStages - 1.  Packs of 2 bytes (rows of 16-bit elements that do
-// not start on 4 bytes) cannot be copied that way and are loaded in place.
+// under the loads of the next kStages - 1.
 // ---------------------------------------------------------------------------
 constexpr int kWide = 128;  // threads of a team that is a CTA
 
 template <int TEAM>
 constexpr int kCtaThreads = TEAM > 32 ? TEAM : kThreads;
 
-// Threads an SM is to hold at once: what the registers are cut to.
-template <int E, int V>
-constexpr int kForwardThreads = V * E <= 8 ? 1024 : V * E <= 16 ? 768 : 512;
-template <int KIND, int E, int V>
-constexpr int kBackwardThreads = KIND == kUnit ? kForwardThreads<E, V> : V * E <= 8 ? 768 : 512;
+// Threads an SM is to hold at once: what the registers are cut to.  With wide packs the
+// ring keeps enough bytes in flight for fewer threads with more registers (layer norm of 130k x 768 bf16 rows,
+// 512 and 768 threads: 71.8 and 76.4 us; with teams of a CTA and four packs, which wait at barriers, 24k x
+// 4096: 136 and 106 us); narrow packs are short of instructions and want the threads (200k x 500: 198 and 172).
+template <int E, int TEAM, int V>
+constexpr int kForwardThreads = V * E <= 8                               ? 1024
+                                : E < 4                                  ? (V * E <= 16 ? 1024 : 768)
+                                : V * E <= 16                            ? 768
+                                : E == 8 && TEAM == kWide                ? 768
+                                                                         : 512;
+template <int KIND, int E, int TEAM, int V>
+constexpr int kBackwardThreads =
+    KIND == kUnit ? (V * E <= 8 ? 1024 : V * E <= 16 ? 768 : 512) : V * E <= 8 ? 768 : 512;
 
-template <typename T, int E>
-constexpr bool kRing = sizeof(T) * E >= 4;
+// How a row's elements get into the ring: a thread's own packs of 16 or 4 bytes; for rows of
+// 16-bit elements that start and end anywhere, the 4-byte words around them, which
+// the lanes of a warp read from each other; or not at all (such rows shared by a CTA).
+enum Staging : int { kInPlace = 0, kPacks = 1, kWords = 2 };
+template <typename T, int E, int TEAM>
+constexpr Staging kStaging = sizeof(T) * E >= 4 ? kPacks : TEAM == 32 ? kWords : kInPlace;
 
 constexpr int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
 
 // Rows in the ring (one of them in use): as many as 200 KB of shared memory hold, 2 to 4.
 template <typename T, int E, int TEAM, int V, int TENSORS, int SM_THREADS>
 constexpr int kStages = clamp_int(200 * 1024 / (SM_THREADS * V * E * (int)sizeof(T) * TENSORS), 2, 4);
+// Bytes of one tensor's part of a stage, all threads of the CTA.
+template <typename T, int E, int TEAM, int V>
+constexpr int kPartBytes = kStaging<T, E, TEAM> == kWords ? kCtaThreads<TEAM> / 32 * (64 * V + 16)
+                                                          : kCtaThreads<TEAM> * V * E * (int)sizeof(T);
 template <typename T, int E, int TEAM, int V, int TENSORS, int SM_THREADS>
-constexpr int kRingBytes =
-    kRing<T, E> ? kStages<T, E, TEAM, V, TENSORS, SM_THREADS> * kCtaThreads<TEAM> * V * E * (int)sizeof(T) * TENSORS : 0;
+constexpr int kRingBytes = kStaging<T, E, TEAM> == kInPlace
+                               ? 0
+                               : kStages<T, E, TEAM, V, TENSORS, SM_THREADS> * TENSORS * kPartBytes<T, E, TEAM, V>;
 
 // The column sums at the end of the backward kernel take the ring's place: element e
 // of a pack lies e * kSumPitch on, which meets no bank twice, written or read.
@@ -278,7 +298,7 @@ constexpr int kSumBytes = 2 * (kCtaThreads<TEAM> / TEAM) * E * kSumPitch<E, TEAM
 // What lies before the weights in the backward kernel's shared memory.
 template <typename T, int KIND, int E, int TEAM, int V>
 constexpr int kBackwardBytes = [] {
-  const int ring = kRingBytes<T, E, TEAM, V, 2, kBackwardThreads<KIND, E, V>>;
+  const int ring = kRingBytes<T, E, TEAM, V, 2, kBackwardThreads<KIND, E, TEAM, V>>;
   const int sums = KIND == kLayer ? kSumBytes<E, TEAM> : 0;
   return ring > sums ? ring : sums;
 }();
@@ -332,26 +352,62 @@ struct Team {
   }
 };
 
-// One thread's packs of the rows ahead, of TENSORS tensors.
-template <typename T, int E, int TEAM, int V, int TENSORS, int STAGES>
+// The rows ahead, of TENSORS tensors.
+template <typename T, int E, int TEAM, int V, int TENSORS>
 struct Ring {
+  static constexpr Staging kHow = kStaging<T, E, TEAM>;
   static constexpr int kBytes = E * (int)sizeof(T);
   static constexpr int kCta = kCtaThreads<TEAM>;
+  static constexpr int kPart = kPartBytes<T, E, TEAM, V>;
   char* mine;
   int lane;
-  __device__ __forceinline__ Ring(char* shared) : mine(shared + threadIdx.x * kBytes), lane(threadIdx.x % TEAM) {}
-  __device__ __forceinline__ char* at(int stage, int tensor, int v) const {
-    return mine + ((stage * TENSORS + tensor) * V + v) * (kCta * kBytes);
+  __device__ __forceinline__ Ring(char* shared)
+      : mine(shared + (kHow == kWords ? (threadIdx.x >> 5) * (64 * V + 16) : threadIdx.x * kBytes)),
+        lane(threadIdx.x % TEAM) {}
+  __device__ __forceinline__ char* at(int stage, int tensor) const {
+    return mine + (stage * TENSORS + tensor) * kPart;
   }
-  __device__ __forceinline__ void copy(int stage, int tensor, const T* row, int dim) const {
+  // Before a stage is filled again: in kWords other lanes have read it.
+  __device__ __forceinline__ void reuse() const {
+    if (kHow == kWords) __syncwarp();
+  }
+  __device__ __forceinline__ void filled() const {
+    if (kHow == kWords) __syncwarp();
+  }
+  // `edge`: the row is the first or last of the tensor, whose outer words are not whole.
+  __device__ __forceinline__ void copy(int stage, int tensor, const T* row, int dim, bool edge) const {
+    if constexpr (kHow == kWords) {
+      const int odd = (int)((uintptr_t)row >> 1) & 1, elements = dim + odd, words = (elements + 1) >> 1;
+      const T* from = row - odd;
+      char* to = at(stage, tensor);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int c = (lane + TEAM * v) * E;
-      if (c < dim) copy_async<kBytes>(at(stage, tensor, v), row + c);
+      for (int v = 0; v <= V / 2; ++v) {
+        const int k = lane + 32 * v;
+        if (k >= words) break;
+        const bool torn = edge && ((k == 0 && odd) || (k == words - 1 && (elements & 1)));
+        if (!torn) {
+          copy_async<4>(to + 4 * k, from + 2 * k);
+        } else {
+          if (k > 0 || !odd) reinterpret_cast<T*>(to)[2 * k] = from[2 * k];
+          if (2 * k + 1 < elements) reinterpret_cast<T*>(to)[2 * k + 1] = from[2 * k + 1];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int c = (lane + TEAM * v) * E;
+        if (c < dim) copy_async<kBytes>(at(stage, tensor) + v * (kCta * kBytes), row + c);
+      }
     }
   }
-  __device__ __forceinline__ Pack<T, E> pack(int stage, int tensor, int v) const {
-    return load_pack<T, E>(at(stage, tensor, v));
+  // Pack v of this thread; `row` is where the row was copied from.
+  __device__ __forceinline__ Pack<T, E> pack(int stage, int tensor, int v, const T* row) const {
+    if constexpr (kHow == kWords) {
+      const int odd = (int)((uintptr_t)row >> 1) & 1;
+      return load_pack<T, E>(reinterpret_cast<const T*>(at(stage, tensor)) + odd + lane + 32 * v);
+    } else {
+      return load_pack<T, E>(at(stage, tensor) + v * (kCta * kBytes));
+    }
   }
 };
 
@@ -371,34 +427,37 @@ struct Turn {
 };
 
 template <typename T, int KIND, int E, int TEAM, int V>
-__global__ void __launch_bounds__(kCtaThreads<TEAM>, kForwardThreads<E, V> / kCtaThreads<TEAM>)
+__global__ void __launch_bounds__(kCtaThreads<TEAM>, kForwardThreads<E, TEAM, V> / kCtaThreads<TEAM>)
 forward_rows_kernel(const T* __restrict__ tokens, const __grid_constant__ Rows t, Affine weight, Affine bias,
                     T* __restrict__ out, float* __restrict__ mean, float* __restrict__ rstd, float eps) {
-  constexpr int S = kRing<T, E> ? kStages<T, E, TEAM, V, 1, kForwardThreads<E, V>> : 1;
+  constexpr Staging kHow = kStaging<T, E, TEAM>;
+  constexpr int S = kHow != kInPlace ? kStages<T, E, TEAM, V, 1, kForwardThreads<E, TEAM, V>> : 1;
   extern __shared__ __align__(16) char shared[];
   __shared__ float words[TEAM > 32 ? TEAM / 8 : 1];
   Team<TEAM> team(words);
-  Ring<T, E, TEAM, V, 1, S> ring(shared);
+  const Ring<T, E, TEAM, V, 1> ring(shared);
   const int lane = threadIdx.x % TEAM;
   const float per = 1.0f / t.dim, least = least_square(eps);
   const Turn<TEAM> turn(t);
   constexpr int R = Turn<TEAM>::kRows;
 
-  Walker ahead;
+  Walker ahead, here;
   if (turn.begin < turn.end) ahead.find(t, turn.begin);
+  here = ahead;
   const auto copy = [&](int stage, int32_t row) {
     if (row < turn.end) {
       ahead.seek(t, row);
-      ring.copy(stage, 0, tokens + ahead.from(t, row), t.dim);
+      const int64_t from = ahead.from(t, row);
+      ring.copy(stage, 0, tokens + from, t.dim, from == 0 || from == t.last());
     }
     copies_commit();
   };
-  if constexpr (kRing<T, E>) {
+  if constexpr (kHow != kInPlace) {
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) copy(i, turn.begin + turn.mine + i * R);
   }
   const int packs = (t.dim + E - 1) / E;
-  float* const after = reinterpret_cast<float*>(shared + kRingBytes<T, E, TEAM, V, 1, kForwardThreads<E, V>>);
+  float* const after = reinterpret_cast<float*>(shared + kRingBytes<T, E, TEAM, V, 1, kForwardThreads<E, TEAM, V>>);
   const Wide<E> w{after, packs}, b{after + packs * E, packs};
   if constexpr (KIND == kLayer) {
     w.template fill<T>(weight, t.dim, 1.0f);
@@ -409,11 +468,16 @@ forward_rows_kernel(const T* __restrict__ tokens, const __grid_constant__ Rows t
   for (int32_t at = turn.begin; at < turn.end; at += R) {
     const int32_t row = at + turn.mine;
     const bool there = row < turn.end;
-    if constexpr (kRing<T, E>) {
+    if constexpr (kHow != kInPlace) {
+      ring.reuse();
       copy(stage == 0 ? S - 1 : stage - 1, row + (S - 1) * R);
       copies_wait<S - 1>();
-    } else if (there) {
-      ahead.seek(t, row);
+      ring.filled();
+    }
+    const T* x = tokens;
+    if (kHow != kPacks && there) {
+      here.seek(t, row);
+      x += here.from(t, row);
     }
     float f[V][E];
     float s = 0.f, ss = 0.f;
@@ -421,8 +485,8 @@ forward_rows_kernel(const T* __restrict__ tokens, const __grid_constant__ Rows t
     for (int v = 0; v < V; ++v) {
       const int c = (lane + TEAM * v) * E;
       if (there && c < t.dim) {
-        if constexpr (kRing<T, E>) expand(ring.pack(stage, 0, v), f[v]);
-        else expand(load_pack<T, E>(tokens + ahead.from(t, row) + c), f[v]);
+        if constexpr (kHow != kInPlace) expand(ring.pack(stage, 0, v, x), f[v]);
+        else expand(load_pack<T, E>(x + c), f[v]);
       } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) f[v][e] = 0.f;
@@ -533,17 +597,18 @@ __device__ __forceinline__ void zero_padding(const Rows& t, T* grad_tokens, int6
 // The row's packs are read twice from the ring (once for the sums, once for the result):
 // the registers go to the column sums.
 template <typename T, int KIND, int E, int TEAM, int V>
-__global__ void __launch_bounds__(kCtaThreads<TEAM>, kBackwardThreads<KIND, E, V> / kCtaThreads<TEAM>)
+__global__ void __launch_bounds__(kCtaThreads<TEAM>, kBackwardThreads<KIND, E, TEAM, V> / kCtaThreads<TEAM>)
 backward_rows_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, const __grid_constant__ Rows t,
                      Affine weight, const float* __restrict__ mean, const float* __restrict__ rstd,
                      T* __restrict__ grad_tokens, float* __restrict__ partial, float eps) {
   constexpr int kCta = kCtaThreads<TEAM>;
-  constexpr int S = kRing<T, E> ? kStages<T, E, TEAM, V, 2, kBackwardThreads<KIND, E, V>> : 1;
+  constexpr Staging kHow = kStaging<T, E, TEAM>;
+  constexpr int S = kHow != kInPlace ? kStages<T, E, TEAM, V, 2, kBackwardThreads<KIND, E, TEAM, V>> : 1;
   constexpr int kFixed = kBackwardBytes<T, KIND, E, TEAM, V>;
   extern __shared__ __align__(16) char shared[];
   __shared__ float words[TEAM > 32 ? TEAM / 8 : 1];
   Team<TEAM> team(words);
-  Ring<T, E, TEAM, V, 2, S> ring(shared);
+  const Ring<T, E, TEAM, V, 2> ring(shared);
   const int lane = threadIdx.x % TEAM;
   const float per = 1.0f / t.dim, least = least_square(eps);
   float dw[KIND == kLayer ? V : 1][E], db[KIND == kLayer ? V : 1][E];
@@ -561,12 +626,13 @@ backward_rows_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, c
   const auto copy = [&](int stage, int32_t row) {
     if (row < turn.end) {
       ahead.seek(t, row);
-      ring.copy(stage, 0, tokens + ahead.from(t, row), t.dim);
-      ring.copy(stage, 1, grad + (int64_t)row * t.dim, t.dim);
+      const int64_t from = ahead.from(t, row);
+      ring.copy(stage, 0, tokens + from, t.dim, from == 0 || from == t.last());
+      ring.copy(stage, 1, grad + (int64_t)row * t.dim, t.dim, row == 0 || row == t.rows - 1);
     }
     copies_commit();
   };
-  if constexpr (kRing<T, E>) {
+  if constexpr (kHow != kInPlace) {
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) copy(i, turn.begin + turn.mine + i * R);
   }
@@ -593,19 +659,23 @@ backward_rows_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, c
         r = rstd[row];
       }
     }
-    if constexpr (kRing<T, E>) {
+    if constexpr (kHow != kInPlace) {
+      ring.reuse();
       copy(stage == 0 ? S - 1 : stage - 1, row + (S - 1) * R);
       copies_wait<S - 1>();
+      ring.filled();
     }
+    const T* const x_row = tokens + (kHow != kPacks && there ? here.from(t, row) : 0);
+    const T* const g_row = grad + (there ? (int64_t)row * t.dim : 0);
     // pack v of the row and of its gradient
     const auto packs_of = [&](int v, float (&x)[E], float (&g)[E]) {
-      if constexpr (kRing<T, E>) {
-        expand(ring.pack(stage, 0, v), x);
-        expand(ring.pack(stage, 1, v), g);
+      if constexpr (kHow != kInPlace) {
+        expand(ring.pack(stage, 0, v, x_row), x);
+        expand(ring.pack(stage, 1, v, g_row), g);
       } else {
         const int c = (lane + TEAM * v) * E;
-        expand(load_pack<T, E>(tokens + here.from(t, row) + c), x);
-        expand(load_pack<T, E>(grad + (int64_t)row * t.dim + c), g);
+        expand(load_pack<T, E>(x_row + c), x);
+        expand(load_pack<T, E>(g_row + c), g);
       }
     };
     T* const dx = grad_tokens + (there ? here.slot(t, row) * t.dim : 0);
