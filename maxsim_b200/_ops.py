@@ -304,24 +304,24 @@ def sample_rows(scores: torch.Tensor, uniforms: torch.Tensor, n: int, temperatur
 NORM_LAYER, NORM_UNIT = 0, 1
 
 
-def norm_rows(kind: int, tokens: torch.Tensor, strides, shape, offsets, packed_rows: int, weight, bias,
-              eps: float, want_stats: bool):
-    """Normalise the rows of ``tokens``: ``shape`` is ``(n_segments, L_max, dim)``
-    and ``strides`` the element strides of its first two dimensions (the last
-    is contiguous).  With ``offsets [n_segments + 1]`` int32 the rows that count
-    are written back to back.  Returns ``(out [packed_rows, dim], stats)``; the
-    statistics ``[2, packed_rows]`` fp32 (means, then reciprocal standard
-    deviations) are None unless asked for (layer norm only)."""
-    dev = tokens.device
-    n, L, dim = shape
-    out = tokens.new_empty((packed_rows, dim))
+def norm_rows(kind: int, tokens: torch.Tensor, call, offsets, weight, bias, eps: float, out_shape, want_stats: bool):
+    """Normalise the rows of ``tokens``.  ``call`` is ``(stride of a segment,
+    stride of a row, n_segments, L_max, dim, packed_rows)``, the strides in
+    elements; the last dimension is contiguous.  With ``offsets [n_segments + 1]``
+    int32 the rows that count are written back to back.  Returns ``(out, stats)``:
+    ``out`` of ``packed_rows`` rows in ``out_shape``; the statistics ``[2, packed_rows]``
+    fp32 (means, then reciprocal standard deviations) are None unless asked for
+    (layer norm only)."""
+    segment_stride, row_stride, n, L, dim, packed_rows = call
+    out = tokens.new_empty(out_shape)
     stats = tokens.new_empty((2, packed_rows), dtype=torch.float32) if want_stats else None
-    at = _ptr(stats) if want_stats else 0
-    with _on_device(dev):
+    at = stats.data_ptr() if want_stats else 0
+    with _on_device(tokens.device):
         rc = load_library().maxsim_b200_norm_rows(
-            kind, _ptr(tokens), strides[0], strides[1], offsets.data_ptr() if offsets is not None else 0,
-            _opt(weight), _opt(bias), _ptr(out), at, at + 4 * packed_rows if at else 0, n, L, dim, packed_rows, eps,
-            _code(tokens), _code(weight) if weight is not None else 0, _stream_ptr())
+            kind, tokens.data_ptr(), segment_stride, row_stride, 0 if offsets is None else offsets.data_ptr(),
+            0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(),
+            at, at + 4 * packed_rows if at else 0, n, L, dim, packed_rows, eps,
+            _code(tokens), 0 if weight is None else _code(weight), _stream_ptr())
     _check(rc, "maxsim_b200_norm_rows")
     return out, stats
 
@@ -332,28 +332,30 @@ def _norm_workspace(device_index, n: int, L: int, dim: int) -> int:
     return load_library().maxsim_b200_norm_rows_workspace(n, L, dim)
 
 
-def norm_rows_backward(kind: int, grad: torch.Tensor, tokens: torch.Tensor, strides, shape, offsets,
-                       packed_rows: int, weight, stats, eps: float, want_tokens: bool, want_weight: bool,
-                       want_bias: bool):
+def norm_rows_backward(kind: int, grad: torch.Tensor, tokens: torch.Tensor, call, offsets, weight, stats, eps: float,
+                       tokens_shape, want_weight: bool, want_bias: bool):
     """The gradients of :func:`norm_rows` that are wanted, else None:
-    ``(grad_tokens [n_segments * L_max * dim], grad_weight [dim], grad_bias
-    [dim])`` from the contiguous ``grad [packed_rows, dim]``."""
+    ``(grad_tokens [n_segments * L_max rows in tokens_shape, which is None when
+    it is not wanted], grad_weight [dim], grad_bias [dim])`` from the contiguous
+    ``grad`` of ``packed_rows`` rows."""
+    segment_stride, row_stride, n, L, dim, packed_rows = call
     dev = tokens.device
-    n, L, dim = shape
-    dx = tokens.new_empty((n * L * dim,)) if want_tokens else None
+    dx = None if tokens_shape is None else tokens.new_empty(tokens_shape)
     dw = torch.empty_like(weight) if want_weight else None
     db = torch.empty_like(weight) if want_bias else None
-    at = _opt(stats)
+    at = 0 if stats is None else stats.data_ptr()
     with _on_device(dev):
         work, size = None, 0
         if want_weight or want_bias:
             size = _norm_workspace(dev.index, n, L, dim)
             work = tokens.new_empty((size,), dtype=torch.uint8)
         rc = load_library().maxsim_b200_norm_rows_backward(
-            kind, _ptr(grad), _ptr(tokens), strides[0], strides[1],
-            offsets.data_ptr() if offsets is not None else 0, _opt(weight), at, at + 4 * packed_rows if at else 0,
-            _opt(dx), _opt(dw), _opt(db), _opt(work), size, n, L, dim, packed_rows, eps,
-            _code(tokens), _code(weight) if weight is not None else 0, _stream_ptr())
+            kind, grad.data_ptr(), tokens.data_ptr(), segment_stride, row_stride,
+            0 if offsets is None else offsets.data_ptr(), 0 if weight is None else weight.data_ptr(),
+            at, at + 4 * packed_rows if at else 0, 0 if dx is None else dx.data_ptr(),
+            0 if dw is None else dw.data_ptr(), 0 if db is None else db.data_ptr(),
+            0 if work is None else work.data_ptr(), size, n, L, dim, packed_rows, eps,
+            _code(tokens), 0 if weight is None else _code(weight), _stream_ptr())
     _check(rc, "maxsim_b200_norm_rows_backward")
     return dx, dw, db
 

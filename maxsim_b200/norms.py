@@ -31,45 +31,30 @@ __all__ = ["layer_norm", "pack_layer_norm", "unit_norm", "pack_unit_norm"]
 _eager = torch.compiler.disable
 
 
-def _two_strides(t: torch.Tensor):
-    """``t [..., dim]`` as ``(tensor, (n, L), (stride_n, stride_L))``: rows the
-    kernels can walk with two strides; copied only when it takes more than two."""
-    dim = t.shape[-1]
-    if t.stride(-1) == 1 or dim == 1:
-        if t.dim() == 2:
-            return t, (1, t.shape[0]), (0, t.stride(0))
-        if t.dim() == 3:
-            return t, (t.shape[0], t.shape[1]), (t.stride(0), t.stride(1))
-    t = t.contiguous()
-    return t, (1, t.numel() // dim if dim else 0), (0, dim)
-
-
-def _forward(kind, tokens, weight, bias, offsets, total, eps, want_stats):
-    """``offsets`` None: rows in, rows out.  Returns the result and what the
-    backward pass needs."""
-    if offsets is None:
-        src, (n, L), strides = _two_strides(tokens)
-        total = n * L
-    else:
-        src = tokens if tokens.stride(2) == 1 else tokens.contiguous()
-        n, L = src.shape[:2]
-        strides = (src.stride(0), src.stride(1))
-    call = (strides, (n, L, tokens.shape[-1]), offsets, total)
-    w = weight.contiguous() if weight is not None else None
-    b = bias.contiguous() if bias is not None else None
-    out, stats = _ops.norm_rows(kind, src, *call, w, b, eps, want_stats)
-    return out if offsets is not None else out.view(tokens.shape), src, w, stats, call
+def _rows(tokens: torch.Tensor):
+    """``tokens [..., dim]`` as ``(tensor, (stride, stride, n, L, dim, n * L))``: rows
+    the kernels can walk with two strides; copied only when it takes more than two."""
+    shape, dim = tokens.shape, tokens.shape[-1]
+    if len(shape) in (2, 3) and (dim == 1 or tokens.stride(-1) == 1):
+        if len(shape) == 2:
+            return tokens, (0, tokens.stride(0), 1, shape[0], dim, shape[0])
+        return tokens, (tokens.stride(0), tokens.stride(1), shape[0], shape[1], dim, shape[0] * shape[1])
+    tokens = tokens.detach().contiguous()
+    rows = tokens.numel() // dim
+    return tokens, (0, dim, 1, rows, dim, rows)
 
 
 class _NormFn(torch.autograd.Function):
-    """The statistics of a layer norm are saved for the backward pass; a unit
-    row's length is taken again from the row."""
+    """``call`` is ``(kind, source rows, their strides and sizes, offsets, eps,
+    shape of the result)``.  The statistics of a layer norm are saved for the
+    backward pass; a unit row's length is taken again from the row."""
 
     @staticmethod
-    def forward(ctx, kind, tokens, weight, bias, offsets, total, eps):
-        out, src, w, stats, call = _forward(kind, tokens, weight, bias, offsets, total, eps, kind == _ops.NORM_LAYER)
-        ctx.save_for_backward(src, w, stats, offsets)
-        ctx.call = (kind, call[0], call[1], call[3], eps, tokens.shape)
+    def forward(ctx, tokens, weight, bias, call):
+        kind, src, rows, offsets, eps, out_shape = call
+        out, stats = _ops.norm_rows(kind, src, rows, offsets, weight, bias, eps, out_shape, kind == _ops.NORM_LAYER)
+        ctx.save_for_backward(src, weight, stats, offsets)
+        ctx.call = (kind, rows, eps, tokens.shape)
         return out
 
     @staticmethod
@@ -80,22 +65,31 @@ class _NormFn(torch.autograd.Function):
 
 
 def _backward(ctx, grad):
-    src, w, stats, offsets = ctx.saved_tensors
-    kind, strides, shape, total, eps, token_shape = ctx.call
-    needs = ctx.needs_input_grad
-    dx, dw, db = _ops.norm_rows_backward(kind, grad.contiguous(), src, strides, shape, offsets, total, w, stats, eps,
-                                         needs[1], needs[2], needs[3])
-    return None, dx.view(token_shape) if dx is not None else None, dw, db, None, None, None
+    src, weight, stats, offsets = ctx.saved_tensors
+    kind, rows, eps, token_shape = ctx.call
+    want_tokens, want_weight, want_bias, _ = ctx.needs_input_grad
+    return *_ops.norm_rows_backward(kind, grad.contiguous(), src, rows, offsets, weight, stats, eps,
+                                    token_shape if want_tokens else None, want_weight, want_bias), None
 
 
 _backward_once = once_differentiable(_backward)
 
 
 def _apply(kind, tokens, weight, bias, offsets, total, eps):
+    """``offsets`` None: rows in, rows out."""
+    if offsets is None:
+        src, rows = _rows(tokens)
+        out_shape = tokens.shape
+    else:
+        src = tokens if tokens.stride(2) == 1 else tokens.detach().contiguous()
+        n, L, dim = src.shape
+        rows, out_shape = (src.stride(0), src.stride(1), n, L, dim, total), (total, dim)
+    weight = weight if weight is None else weight.contiguous()
+    bias = bias if bias is None else bias.contiguous()
     if torch.is_grad_enabled() and (tokens.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
-        return _NormFn.apply(kind, tokens, weight, bias, offsets, total, eps)
-    return _forward(kind, tokens, weight, bias, offsets, total, eps, False)[0]
+        return _NormFn.apply(tokens, weight, bias, (kind, src, rows, offsets, eps, out_shape))
+    return _ops.norm_rows(kind, src, rows, offsets, weight, bias, eps, out_shape, False)[0]
 
 
 def _check(name: str, tokens, weight, bias, eps) -> None:
