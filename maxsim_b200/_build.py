@@ -22,7 +22,7 @@ CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libmaxsim_b200.so"
 STAMP_PATH = PKG_DIR / "libmaxsim_b200.stamp"
 
-SOURCES = ["abi.cu", "norm.cu", "sample.cu"]
+SOURCES = ["abi.cu", "norm_forward.cu", "norm_backward.cu", "sample.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

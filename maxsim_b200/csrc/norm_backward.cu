@@ -1,0 +1,122 @@
+// extern "C" entry points of the gradients of the row normalisation operators.
+#include "norm_host.cuh"
+
+namespace maxsim {
+namespace {
+
+// Rows of the partial sums of the weight's gradient: one for each CTA of a layer norm's
+// backward kernel, at most 512 threads or four CTAs on an SM.
+int grad_slabs(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>(rows, 4 * sm_count())); }
+
+struct Backward {
+  static constexpr bool kSums = true;
+  const void* grad;
+  const void* tokens;
+  norm::Rows t;
+  norm::Affine weight;
+  const float* mean;
+  const float* rstd;
+  void* grad_tokens;
+  float* partial;  // null: no sums are wanted
+  float eps;
+  cudaStream_t st;
+  mutable int slabs = 0;  // rows of `partial` that were written
+  bool aligned(int bytes) const {
+    const uintptr_t all = (uintptr_t)grad | (uintptr_t)tokens | (uintptr_t)grad_tokens | (uintptr_t)weight.p;
+    return all % bytes == 0;
+  }
+
+  template <typename T, int KIND, int E, int TEAM, int V>
+  int rows() const {
+    constexpr int threads = norm::kCtaThreads<TEAM>, per_sm = norm::kBackwardThreads<KIND, E, TEAM, V>;
+    constexpr int fixed = norm::kBackwardBytes<T, KIND, E, TEAM, V>;
+    auto kern = norm::backward_rows_kernel<T, KIND, E, TEAM, V>;
+    static std::atomic<unsigned char> configured[kMaxDevices];
+    constexpr int most = fixed + (KIND == norm::kLayer ? norm::Wide<E>::bytes(TEAM * V * E) : 0);
+    static_assert(most <= 227 * 1024, "shared memory of a CTA");
+    if (int rc = ensure_smem(kern, most, configured)) return rc;
+    Split split = share_rows<threads, TEAM>(std::max(t.rows, 1), per_sm / threads);
+    if (t.offsets) {  // few rows in much padding: as many CTAs as its zeros keep busy
+      const int64_t most_ctas = (int64_t)sm_count() * (per_sm / threads);
+      split.grid = (unsigned)std::max<int64_t>(split.grid, std::min(most_ctas, ceil_div((int64_t)t.n_segments * t.L_max, 64)));
+    }
+    slabs = (int)split.grid;
+    const int smem = fixed + (KIND == norm::kLayer ? norm::Wide<E>::bytes(t.dim) : 0);
+    kern<<<split.grid, threads, smem, st>>>((const T*)grad, (const T*)tokens, split.of(t), weight, mean, rstd,
+                                            (T*)grad_tokens, partial, eps);
+    return launch_check("norm backward_rows_kernel");
+  }
+  template <typename T, int KIND>
+  int wide() const {
+    if (grad_tokens) {
+      const Split split = share_rows<norm::kThreads, 32>(std::max(t.rows, 1), 8);
+      norm::backward_wide_kernel<T, KIND><<<split.grid, norm::kThreads, 0, st>>>(
+          (const T*)grad, (const T*)tokens, split.of(t), weight, mean, rstd, (T*)grad_tokens, eps);
+      if (int rc = launch_check("norm backward_wide_kernel")) return rc;
+    }
+    if (!partial) return MAXSIM_OK;
+    slabs = std::min(grad_slabs(t.rows), 64);
+    norm::grad_weight_wide_kernel<T><<<dim3((unsigned)ceil_div(t.dim, norm::kThreads), (unsigned)slabs),
+                                       norm::kThreads, 0, st>>>(
+        (const T*)grad, (const T*)tokens, t, mean, rstd, partial, slabs);
+    return launch_check("norm grad_weight_wide_kernel");
+  }
+};
+
+template <typename W>
+int launch_sum(const Backward& call, void* grad_weight, void* grad_bias) {
+  norm::grad_weight_sum_kernel<W><<<dim3((unsigned)ceil_div(call.t.dim, 32), 2), norm::kSumThreads, 0, call.st>>>(
+      call.partial, call.slabs, call.t.dim, (W*)grad_weight, (W*)grad_bias);
+  return launch_check("norm grad_weight_sum_kernel");
+}
+
+}  // namespace
+}  // namespace maxsim
+
+using namespace maxsim;
+
+extern "C" {
+
+int64_t maxsim_b200_norm_rows_workspace(int64_t n_segments, int64_t L_max, int64_t dim) {
+  if (n_segments <= 0 || L_max <= 0 || dim <= 0 || n_segments > kMaxRows / L_max) return 0;
+  return (int64_t)grad_slabs(n_segments * L_max) * dim * 2 * (int64_t)sizeof(float);
+}
+
+int maxsim_b200_norm_rows_backward(int kind, const void* grad, const void* tokens, int64_t segment_stride,
+                                   int64_t row_stride, const int32_t* offsets, const void* weight,
+                                   const float* mean, const float* rstd, void* grad_tokens, void* grad_weight,
+                                   void* grad_bias, void* workspace, int64_t workspace_bytes,
+                                   int64_t n_segments, int64_t L_max, int64_t dim, int64_t packed_rows,
+                                   double eps, int dtype, int weight_dtype, void* stream) {
+  norm::Rows t;
+  if (int rc = check_rows(kind, n_segments, L_max, dim, packed_rows, segment_stride, row_stride, offsets, eps, &t))
+    return rc;
+  if (kind == norm::kUnit && (weight || grad_weight || grad_bias))
+    return fail(MAXSIM_EINVAL, "unit rows have no weights");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool sums = grad_weight || grad_bias;
+  if (int rc = check_types(dtype, weight_dtype)) return rc;
+  if (int rc = check_bases({grad, tokens, grad_tokens}, dtype, {weight, grad_weight, grad_bias}, weight_dtype)) return rc;
+  if (n_segments * L_max == 0) {  // no rows: the sums are zero
+    const size_t bytes = (size_t)dim * element_size(weight_dtype);
+    if (grad_weight) MAXSIM_CUDA(cudaMemsetAsync(grad_weight, 0, bytes, st));
+    if (grad_bias) MAXSIM_CUDA(cudaMemsetAsync(grad_bias, 0, bytes, st));
+    return MAXSIM_OK;
+  }
+  if (!grad_tokens && !sums) return MAXSIM_OK;
+  if (!tokens || (!grad && packed_rows > 0)) return fail(MAXSIM_EINVAL, "null pointer argument");
+  if (kind == norm::kLayer && packed_rows > 0 && (!mean || !rstd)) return fail(MAXSIM_EINVAL, "null pointer argument");
+  if (sums && (!workspace || workspace_bytes < maxsim_b200_norm_rows_workspace(n_segments, L_max, dim)))
+    return fail(MAXSIM_EWORKSPACE, "workspace missing or smaller than maxsim_b200_norm_rows_workspace says");
+  const Backward call{grad, tokens, t, {weight, weight_dtype == MAXSIM_F32}, mean, rstd, grad_tokens,
+                      sums ? static_cast<float*>(workspace) : nullptr, (float)eps, st};
+  if (int rc = launch(kind, dtype, call)) return rc;
+  if (!sums) return MAXSIM_OK;
+  switch (weight_dtype) {
+    case MAXSIM_F32: return launch_sum<float>(call, grad_weight, grad_bias);
+    case MAXSIM_F16: return launch_sum<__half>(call, grad_weight, grad_bias);
+    default: return launch_sum<__nv_bfloat16>(call, grad_weight, grad_bias);
+  }
+}
+
+}  // extern "C"

@@ -6,7 +6,7 @@
 // "score descending, index ascending" every filter keeps a prefix:
 //   top-k   the first k
 //   top-p   of those, the ones before which less than p of their mass lies
-//   min-p   w_i >= min_p (times the best weight, which is 1)
+//   min-p   a_i >= log(min_p): w_i >= min_p times the best weight, which is 1
 // n candidates are drawn without replacement: the n largest of
 // a_i - log(-log u_i) among the kept, largest first, equal ones by lowest
 // index.  -log(u_i) / w_i is the arrival time of an exponential clock of rate
@@ -109,15 +109,13 @@ __device__ __forceinline__ uint32_t key_of(float v) {
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
-// The smallest finite score whose weight is at least `weight` (or whose exponent is at least
-// `least`, with weight 0): weights rise with scores, so one comparison of floats
-// decides afterwards.  `guess` is a few roundings away as a number, which near zero can be a great
-// many floats: steps that double, then halving, some 60 tries at the very most.
-__device__ __noinline__ float first_score(float best, double T, double least, double weight, double guess) {
-  const auto holds = [&](uint32_t key) {
-    const double a = exponent(value_of(key), best, T);
-    return weight > 0.0 ? exp(a) >= weight : a >= least;
-  };
+// The smallest finite score whose exponent is at least `least` (<= 0): exponents rise with
+// scores, so one comparison of floats decides afterwards.  best + least * T is a few roundings
+// away as a number, which near zero can be a great many floats: steps that double, then
+// halving, some 60 tries at the very most.
+__device__ __noinline__ float first_score(float best, double T, double least) {
+  const auto holds = [&](uint32_t key) { return exponent(value_of(key), best, T) >= least; };
+  const double guess = (double)best + least * T;
   const uint32_t lowest = key_of(-3.402823466e38f), top = key_of(best);  // holds(top)
   uint32_t x = guess >= best ? top : guess > -3.4e38 ? key_of(__double2float_ru(guess)) : lowest;
   uint32_t out = x, in = x;  // !holds(out), holds(in)
@@ -346,7 +344,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   // candidates are the scores from `first` on (false for NaN and -inf)
   const float first = (double)least - (double)best > -699.0 * T
                           ? least
-                          : first_score(best, T, kLeast, 0.0, (double)best + kLeast * T);
+                          : first_score(best, T, kLeast);
 
   // The filters keep a prefix: scores above `cut`, and those equal to it up to index `cut_index`.
   float cut = -INFINITY;
@@ -547,8 +545,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   }
   const double least_share = A.min_p.at(row);
   const bool by_share = least_share > 0.0 && least_share <= 1.0;
-  const float floor_score =
-      by_share ? fmaxf(first, first_score(best, T, 0.0, least_share, (double)best + T * log(least_share))) : first;
+  const float floor_score = by_share ? fmaxf(first, first_score(best, T, log(least_share))) : first;
   const auto kept = [&](float v, int i) { return v >= floor_score && inside(v, i); };
 
   // The race in 32 bits: lower bounds.  -log u is a polynomial in 1 - u where u is near 1 (to

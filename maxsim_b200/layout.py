@@ -161,7 +161,10 @@ def _per_row(name: str, value, rows: int, dtype, device, least: float, most: flo
             raise RuntimeError(f"{name} must be on the scores' device {device}; got {value.device}")
         if value.is_floating_point() != (dtype == torch.float32) or value.dtype == torch.bool:
             raise TypeError(f"{name} must hold {'floats' if dtype == torch.float32 else 'integers'}; got {value.dtype}")
-        return value.detach().to(dtype).contiguous()
+        value = value.detach()
+        if value.dtype == torch.int64:  # anything past 32 bits keeps all
+            value = value.clamp(min=0, max=2 ** 31 - 1)
+        return value.to(dtype).contiguous()
     if not least < value <= most:
         raise ValueError(f"{name} must be in ({least}, {most}]; got {value}")
     return value

@@ -410,8 +410,8 @@ def sample_candidates(scores, uniforms, n, temperature=1.0, top_k=0, top_p=1.0, 
                 before += w[size]
                 size += 1
             ids = ids[:size]
-        if 0 < least <= 1:
-            ids = [i for i in ids if np.exp(a[i]) >= least]
+        if 0 < least <= 1:  # exp(a) >= least, without the rounding of exp next to 1
+            ids = [i for i in ids if a[i] >= np.log(least)]
         total = np.exp([a[i] for i in ids]).sum()
         with np.errstate(divide="ignore", invalid="ignore"):
             race = {i: a[i] - np.log(-np.log(uniforms[b, i])) for i in ids}

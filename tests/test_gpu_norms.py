@@ -345,6 +345,98 @@ def test_empty_batches():
     assert y.shape == (0, 16) and off.tolist() == [0]
 
 
+def test_empty_segments_and_short_rows_in_much_padding():
+    """Lengths on the device may be zero; one packed row among thousands of padded ones."""
+    for lens, L in (([0, 3, 0, 0, 5, 0], 7), ([0, 0, 0], 4), ([1] + [0] * 40, 200), ([0] * 33 + [9], 9)):
+        x = rows_of((len(lens), L, 64), torch.bfloat16, L).requires_grad_(True)
+        w = rows_of((64,), torch.float32, 1).requires_grad_(True)
+        T = sum(lens)
+        ln = torch.tensor(lens, device=DEV)
+        y, off = maxsim.pack_layer_norm(x, ln, w, w, total_tokens=T)
+        assert off.tolist() == [0] + np.cumsum(lens).tolist() and y.shape == (T, 64)
+        g = rows_of((T, 64), torch.bfloat16, 2)
+        dx, dw = torch.autograd.grad(y, (x, w), g)
+        valid = torch.arange(L, device=DEV)[None, :] < ln[:, None]
+        assert not dx[~valid].any()
+        if T:
+            check_layer(x.detach()[valid], w, w, None, y, None)
+            assert dx[valid].abs().sum() > 0 and dw.abs().sum() > 0
+        else:
+            assert not dw.any()
+        y, _ = maxsim.pack_unit_norm(x, ln, total_tokens=T)
+        (dx,) = torch.autograd.grad(y, x, g)
+        assert not dx[~valid].any()
+        if T:
+            check_unit(x.detach()[valid], g, y, dx[valid])
+
+
+@pytest.mark.parametrize("dim", [1, 3, 65, 333, 777])
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+def test_odd_rows_at_every_offset(dim, offset):
+    """16-bit rows of odd width that start on any element: neighbouring rows share 4-byte
+    words, the first and the last row have words that reach past the tensor."""
+    N, L = 5, 6
+    base = rows_of((N * L * dim + 8,), torch.bfloat16, dim)
+    base[:offset] = float("nan")           # what lies outside is not used
+    base[offset + N * L * dim:] = float("nan")
+    x = base[offset: offset + N * L * dim].view(N, L, dim).detach().requires_grad_(True)
+    w = rows_of((dim,), torch.bfloat16, 1).requires_grad_(True)
+    g = rows_of((N * L * dim + 1,), torch.bfloat16, 2)[1 - offset % 2:][: N * L * dim].view(N, L, dim)
+    y = maxsim.layer_norm(x, w, w)
+    dx, dw = torch.autograd.grad(y, (x, w), g)
+    check_layer(x, w, w, g, y, (dx, None, None))
+    assert torch.isfinite(dw).all()
+    y = maxsim.unit_norm(x)
+    check_unit(x, g, y, torch.autograd.grad(y, x, g)[0])
+    ln = torch.tensor([6, 1, 3, 2, 6])
+    valid = (torch.arange(L)[None, :] < ln[:, None]).to(DEV)
+    y, _ = maxsim.pack_unit_norm(x, ln)
+    gp = rows_of((18, dim), torch.bfloat16, 3)
+    (dx,) = torch.autograd.grad(y, x, gp)
+    check_unit(x.detach()[valid], gp, y, dx[valid])
+    assert not dx[~valid].any()
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the rows at both ends and around element 2^31."""
+    D, rows = 2048, 1_100_000
+    x = torch.empty((rows, D), device=DEV, dtype=torch.bfloat16)
+    x.normal_(generator=torch.Generator(device=DEV).manual_seed(0))
+    x.requires_grad_(True)
+    w = rows_of((D,), torch.float32, 1, 0.3, 1.0)
+    g = torch.empty_like(x, requires_grad=False).normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    some = torch.tensor([0, 1, 2 ** 20 - 1, 2 ** 20, 2 ** 20 + 1, rows - 2, rows - 1], device=DEV)
+    y = maxsim.layer_norm(x, w)
+    (dx,) = torch.autograd.grad(y, x, g)
+    check_layer(x.detach()[some], w, None, g[some], y.detach()[some], (dx[some], None, None))
+    del y, dx
+    L = 11
+    lens = torch.full((rows // L,), 10)
+    y, off = maxsim.pack_unit_norm(x.view(rows // L, L, D), lens)
+    check_unit(x.detach().view(-1, L, D)[-1, :10], None, y[-10:], None)
+    assert int(off[-1]) == y.shape[0] == rows // L * 10
+
+
+def test_gradients_under_create_graph_and_autocast():
+    x = rows_of((6, 32), torch.float32, 0).requires_grad_(True)
+    y = maxsim.unit_norm(x)
+    (dx,) = torch.autograd.grad(y.sum() + (x ** 3).sum(), x, create_graph=True)  # allowed: only x ** 3 is used twice
+    assert dx.shape == x.shape
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        w = torch.ones(32, device=DEV)
+        assert maxsim.layer_norm(x.detach().bfloat16(), w).dtype == torch.bfloat16
+        assert maxsim.layer_norm(x.detach(), w).dtype == torch.float32
+    with torch.no_grad():
+        assert not maxsim.layer_norm(x).requires_grad
+    x2 = rows_of((6, 32), torch.float32, 0).requires_grad_(True)
+    y = maxsim.unit_norm(x2 * 1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        z = x2 * 1
+        y = maxsim.unit_norm(z)
+        z.add_(1)
+        y.sum().backward()
+
+
 def test_packed_refusals():
     x = torch.zeros(4, 8, 16, device=DEV)
     with pytest.raises(ValueError, match="lengths must be in"):

@@ -119,6 +119,83 @@ def test_uniforms_at_and_outside_their_ends():
     check(s, u, 20, top_k=30, top_p=0.9)
 
 
+def test_many_equal_values():
+    """More equal scores or race values than the kernels list."""
+    C = 5000
+    u = torch.rand(4, C, generator=torch.Generator().manual_seed(0))
+    s = torch.zeros(4, C)
+    s[1, ::2] = -1.0
+    s[2, :100] = 5.0
+    s[3, 4000:] = 2.0
+    for kw in (dict(), dict(top_k=700), dict(top_k=3000, top_p=0.9), dict(top_p=0.37), dict(min_p=0.5), dict(top_p=0.999)):
+        check(s, u, 30, **kw)
+    check(s, torch.full((4, C), 0.25), 30)          # all race values of equal scores equal
+    check(s, torch.full((4, C), 0.25), 1000, top_k=2500)
+    check(s, (u * 4).floor() / 4 + 0.125, 60)
+    got, _ = check(s, torch.full((4, C), 0.25), 5, top_k=700)
+    assert got[0].tolist() == [0, 1, 2, 3, 4] and got[3].tolist() == [4000, 4001, 4002, 4003, 4004]
+
+
+def test_scores_at_every_scale():
+    """Clusters that a linear map of the whole range cannot tell apart, outliers on both
+    sides, values next to zero and at both ends of the type."""
+    g = torch.Generator().manual_seed(1)
+    C = 4096
+    u = torch.rand(8, C, generator=g)
+    s = torch.randn(8, C, generator=g)
+    s[0] = 1.0 + s[0] * 1e-6
+    s[0, 17] = 3e38
+    s[0, 18] = -3e38
+    s[1] = 2.0 ** torch.randint(-140, 120, (C,), generator=g).float()
+    s[2] = s[2] * 1e-40                      # subnormal
+    s[3] = -(2.0 ** torch.randint(-140, 120, (C,), generator=g).float())
+    s[4, ::3] = 0.0
+    s[4, 1::3] = -0.0
+    s[5] = torch.linspace(-3.4e38, 3.4e38, C)
+    s[6] = (s[6] * 3).round()
+    s[7] = 1e9 + (s[7] * 10).round() * 64
+    for T in (1e-38, 1e-3, 0.01, 1.0, 1e30, INF):
+        for kw in (dict(), dict(top_k=300), dict(top_k=1500, top_p=0.7), dict(top_p=0.6), dict(min_p=1.0), dict(min_p=1e-30)):
+            check(s, u, 20, temperature=T, **kw)
+    check(torch.tensor([[7.0, 0.0, 1e-30, -1e-30, 3.5]]), torch.tensor([[0.5, 0.6, 0.7, 0.8, 0.9]]), 5, temperature=0.01)
+    check(torch.zeros(1, 400), torch.rand(1, 400, generator=g), 9, min_p=1.0)
+
+
+def test_uniforms_below_the_normal_range():
+    s, u = scores_of(3, 400, 12)
+    u[0, ::2] = 1e-40
+    u[1, 5] = 1e-45
+    check(s, u, 250)
+    check(s, u, 20, top_k=100)
+
+
+def test_rows_around_the_choices_of_a_launch():
+    """Row counts and widths on both sides of where another number of threads is taken."""
+    for B, C, n in ((593, 40, 5), (800, 300, 130), (600, 2048, 128), (592, 100, 20), (3, 2049, 40), (2, 24576, 40),
+                    (2, 24577, 40), (2, 40960, 40), (2, 40961, 40), (1, 300_001, 9)):
+        s, u = scores_of(B, C, B + C)
+        some = torch.randperm(B, generator=torch.Generator().manual_seed(0))[:3]
+        got, share = maxsim.sample_candidates(s.to(DEV), u.to(DEV), n, temperature=0.6, top_k=C // 2 + 1, top_p=0.95)
+        want, wshare = oracle.sample_candidates(s[some].numpy(), u[some].numpy(), n, 0.6, C // 2 + 1, 0.95)
+        np.testing.assert_array_equal(got[some].cpu().numpy(), want)
+        np.testing.assert_allclose(share[some].cpu().numpy(), wshare, rtol=2.0 ** -23)
+
+
+def test_two_streams_at_once():
+    parts = [tuple(t.to(DEV) for t in scores_of(300, 1500, i)) for i in range(2)]
+    want = [maxsim.sample_candidates(s, u, 10, temperature=0.4, top_p=0.9) for s, u in parts]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in parts]
+    got = [[], []]
+    for _ in range(5):
+        for i, (s, u) in enumerate(parts):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(maxsim.sample_candidates(s, u, 10, temperature=0.4, top_p=0.9))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for run in got[i] for a, b in zip(run, want[i]))
+
+
 def test_one_value_per_row():
     B = 12
     s, u = scores_of(B, 200, 6)
@@ -131,6 +208,7 @@ def test_one_value_per_row():
     check(s, u, 9, temperature=T)
     check(s, u, 9, top_k=k)
     check(s, u, 9, top_k=k.long(), temperature=0.4)
+    check(s, u, 9, top_k=k.long() + 2 ** 33, temperature=0.4)
     check(s, u, 9, top_p=p)
     check(s, u, 9, min_p=m)
     got, _ = check(s, u, 9, temperature=T, top_k=k, top_p=p, min_p=m)

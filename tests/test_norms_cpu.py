@@ -170,6 +170,9 @@ def test_c_entries_refuse_without_touching_a_device():
     assert norm(n=2 ** 20, L=2 ** 20) == -2 and "rows" in error()
     assert norm(n=2 ** 40, L=2 ** 40) == -2
     assert norm(n=0) == 0 and norm(L=0) == 0
+    odd = lambda at, dt: lib.maxsim_b200_norm_rows(0, at, 32, 8, 0, 0, 0, 16, 0, 0, 1, 4, 8, 4, 1e-5, dt, dt, 0)  # noqa: E731
+    assert odd(18, 0) == -1 and "element size" in error() and odd(17, 1) == -1
+    assert norm(dt=0, wdt=1) == -2 and norm(dt=7) == -1 and "dtype" in error()
     assert lib.maxsim_b200_norm_rows_workspace(0, 4, 8) == 0
     back = lambda dw=0, ws=0, nbytes=0, kind=0: lib.maxsim_b200_norm_rows_backward(  # noqa: E731
         kind, 8, 8, 32, 8, 0, 0, 8, 8, 0, dw, 0, ws, nbytes, 1, 4, 8, 4, 1e-5, 0, 0, 0)
