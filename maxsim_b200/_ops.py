@@ -500,8 +500,9 @@ def _groups(key: torch.Tensor, ids32: torch.Tensor, n_bins: int, build: bool = T
     if not build:
         return None
     groups = group_pairs(ids32, n_bins)
-    if len(_GROUP_CACHE) >= _GROUP_CACHE_LIMIT:
-        _GROUP_CACHE.clear()
+    _GROUP_CACHE.pop(id(key), None)
+    while len(_GROUP_CACHE) >= _GROUP_CACHE_LIMIT:  # the oldest only: a call needs two that stay together
+        _GROUP_CACHE.pop(next(iter(_GROUP_CACHE)))
     try:
         _GROUP_CACHE[id(key)] = (weakref.ref(key), key._version, n_bins, groups)
     except TypeError:
