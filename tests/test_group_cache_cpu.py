@@ -12,6 +12,7 @@ def test_a_full_memory_keeps_the_newest_groupings(monkeypatch):
     made = []
     monkeypatch.setattr(_ops, "group_pairs", lambda ids, n: made.append(ids) or object())
     monkeypatch.setattr(_ops, "_GROUP_CACHE", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     ids = [torch.zeros(_ops.GROUP_MIN_PAIRS, dtype=torch.int32) for _ in range(3 * _ops._GROUP_CACHE_LIMIT)]
     for by_document, by_query in zip(ids[::2], ids[1::2]):
         first = _ops._groups(by_document, by_document, 5), _ops._groups(by_query, by_query, 5)
