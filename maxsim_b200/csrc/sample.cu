@@ -53,11 +53,14 @@ int maxsim_b200_sample_rows(const float* scores, int64_t score_stride, const flo
   A.indices = indices;
   A.probabilities = probabilities;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // Threads of a row.  A CTA's barriers and reductions cost the same for few elements as for many: with
-  // more rows than run at once small CTAs get more done (1024 rows of 1024, 16 draws: 17.7 us with 128
-  // threads, 22.3 with 256), with fewer the row itself has to be quick (256 rows of 1000: 12.0 and 10.4 us).
-  if (cols <= 2048 && n <= 128 && rows > 4 * sm_count()) return launch_rows<128, true>(A, st);
-  if (cols <= 2048) return launch_rows<256, true>(A, st);
+  // Threads of a row.  A CTA's barriers and reductions cost the same for few elements as for many:
+  // with more rows than run at once small CTAs get more done, with fewer the row itself has to be quick.
+  // Measured, top-p draws, us with 128 / 256 / 512 threads: 1 x 1000 10.4 / 9.4 / 10.2, 700 x 500 24.6 / 28.9 / 37.9;
+  // 140 x 8000 29.5 / 20.3 / 16.6, 600 x 8000 56.7 / 42.3 / 47.5; 512 x 20000, where shared memory holds two
+  // rows whatever their threads, 123 / 82 / 68.
+  const int sms = sm_count();
+  if (cols <= 2048 && n <= 128 && rows > 4 * sms) return launch_rows<128, true>(A, st);
+  if (cols <= 2048 || (cols <= 8192 && rows > 2 * sms)) return launch_rows<256, true>(A, st);
   if (cols <= 24576) return launch_rows<512, true>(A, st);
   if (cols <= sample::kMostCached) return launch_rows<1024, true>(A, st);
   return launch_rows<1024, false>(A, st);

@@ -171,7 +171,7 @@ def test_uniforms_below_the_normal_range():
 
 def test_rows_around_the_choices_of_a_launch():
     """Row counts and widths on both sides of where another number of threads is taken."""
-    for B, C, n in ((593, 40, 5), (800, 300, 130), (600, 2048, 128), (592, 100, 20), (3, 2049, 40), (2, 24576, 40),
+    for B, C, n in ((593, 40, 5), (800, 300, 130), (600, 2048, 128), (592, 100, 20), (3, 2049, 40), (296, 8192, 9), (297, 8192, 9), (297, 8193, 9), (2, 24576, 40),
                     (2, 24577, 40), (2, 40960, 40), (2, 40961, 40), (1, 300_001, 9)):
         s, u = scores_of(B, C, B + C)
         some = torch.randperm(B, generator=torch.Generator().manual_seed(0))[:3]
