@@ -48,7 +48,7 @@ struct Rows {
   const int32_t* offsets;              // [n_segments + 1], or null
   int32_t n_segments, L_max;
   int32_t rows;   // packed rows: the ones at or beyond are never touched
-  int32_t chunk;  // consecutive packed rows of one unit (a warp, or a CTA)
+  int32_t chunk;  // consecutive packed rows of a CTA
   int32_t dim;
 
   __device__ __forceinline__ int32_t start(int32_t n) const { return offsets ? offsets[n] : n * L_max; }
@@ -60,7 +60,7 @@ struct Rows {
   __device__ __forceinline__ int32_t used() const { return min(rows, start(n_segments)); }
 };
 
-// Walks the packed rows upwards and knows the segment it is in.  A unit looks its first segment up
+// Walks the packed rows upwards and knows the segment it is in.  A warp looks its first segment up
 // once (32 offsets at a time) and then only steps: no division and, within a
 // segment, no load.  Offsets that are none (decreasing, longer than L_max) lead to a
 // token row of the batch, never out of it.
@@ -128,42 +128,95 @@ __device__ __forceinline__ void store_pack(void* p, const Pack<T, E>& x) {
   *reinterpret_cast<U*>(p) = *reinterpret_cast<const U*>(&x);
 }
 
+// The elements of a pack as floats: in pairs, on which one instruction works at a time
+// (the kernels are short of instructions), or one by one.
+struct Pair {
+  unsigned long long bits;
+};
+__device__ __forceinline__ Pair pair_of(float x, float y) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.bits) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ float2 both_of(Pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.bits));
+  return f;
+}
+__device__ __forceinline__ Pair add(Pair a, Pair b) {
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(a.bits) : "l"(b.bits));
+  return a;
+}
+__device__ __forceinline__ Pair mul(Pair a, Pair b) {
+  asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a.bits) : "l"(b.bits));
+  return a;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(a.bits) : "l"(b.bits), "l"(c.bits));
+  return a;
+}
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+__device__ __forceinline__ float mul(float a, float b) { return a * b; }
+__device__ __forceinline__ float fma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float total(Pair p) { const float2 f = both_of(p); return f.x + f.y; }
+__device__ __forceinline__ float total(float f) { return f; }
+__device__ __forceinline__ float most(Pair p) { const float2 f = both_of(p); return fmaxf(fabsf(f.x), fabsf(f.y)); }
+__device__ __forceinline__ float most(float f) { return fabsf(f); }
+template <typename X> __device__ __forceinline__ X splat(float f);
+template <> __device__ __forceinline__ Pair splat<Pair>(float f) { return pair_of(f, f); }
+template <> __device__ __forceinline__ float splat<float>(float f) { return f; }
+
+template <int E>
+using Elem = typename std::conditional<E % 2 == 0, Pair, float>::type;
+template <int E>
+constexpr int kElems = E % 2 == 0 ? E / 2 : 1;
+
 template <typename T, int E>
-__device__ __forceinline__ void expand(const Pack<T, E>& p, float (&f)[E]) {
-  if constexpr (sizeof(T) == 2 && E % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      const uint32_t u = reinterpret_cast<const uint32_t*>(&p)[i];
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) {  // the upper half of a float
-        f[2 * i] = __uint_as_float(u << 16);
-        f[2 * i + 1] = __uint_as_float(u & 0xffff0000u);
-      } else {
-        const float2 both = __half22float2(reinterpret_cast<const __half2&>(u));
-        f[2 * i] = both.x;
-        f[2 * i + 1] = both.y;
-      }
-    }
+__device__ __forceinline__ void expand(const Pack<T, E>& p, Elem<E> (&f)[kElems<E>]) {
+  if constexpr (E % 2 != 0) {
+    f[0] = widen(p.v[0]);
   } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) f[e] = widen(p.v[e]);
+    for (int i = 0; i < E / 2; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        f[i] = pair_of(p.v[2 * i], p.v[2 * i + 1]);
+      } else {
+        const uint32_t u = reinterpret_cast<const uint32_t*>(&p)[i];
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {  // the upper half of a float
+          f[i] = pair_of(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+        } else {
+          const float2 both = __half22float2(reinterpret_cast<const __half2&>(u));
+          f[i] = pair_of(both.x, both.y);
+        }
+      }
+    }
   }
 }
 template <typename T, int E>
-__device__ __forceinline__ Pack<T, E> compress(const float (&f)[E]) {
+__device__ __forceinline__ Pack<T, E> compress(const Elem<E> (&f)[kElems<E>]) {
   Pack<T, E> p;
-  if constexpr (sizeof(T) == 2 && E % 2 == 0) {
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) {
-      if constexpr (std::is_same<T, __nv_bfloat16>::value)
-        reinterpret_cast<__nv_bfloat162*>(&p)[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-      else
-        reinterpret_cast<__half2*>(&p)[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    }
+  if constexpr (E % 2 != 0) {
+    p.v[0] = narrow<T>(f[0]);
   } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) p.v[e] = narrow<T>(f[e]);
+    for (int i = 0; i < E / 2; ++i) {
+      const float2 both = both_of(f[i]);
+      if constexpr (sizeof(T) == 4) {
+        p.v[2 * i] = both.x;
+        p.v[2 * i + 1] = both.y;
+      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        reinterpret_cast<__nv_bfloat162*>(&p)[i] = __floats2bfloat162_rn(both.x, both.y);
+      } else {
+        reinterpret_cast<__half2*>(&p)[i] = __floats2half2_rn(both.x, both.y);
+      }
+    }
   }
   return p;
+}
+
+template <int E>
+__device__ __forceinline__ Pack<float, E> unpacked(const Elem<E> (&f)[kElems<E>]) {
+  return compress<float, E>(f);
 }
 
 // A layer norm's weight or bias: float, or of the rows' type.
@@ -191,12 +244,16 @@ struct Wide {
       words[((e / kPart) * packs + pack) * kPart + e % kPart] = a.p && c < dim ? a.at<T>(c) : none;
     }
   }
-  __device__ __forceinline__ void get(int pack, float (&w)[E]) const {
+  __device__ __forceinline__ void get(int pack, Elem<E> (&w)[kElems<E>]) const {
 #pragma unroll
     for (int i = 0; i < E / kPart; ++i) {
       const Pack<float, kPart> f = load_pack<float, kPart>(words + (i * packs + pack) * kPart);
+      if constexpr (E % 2 != 0) {
+        w[0] = f.v[0];
+      } else {
 #pragma unroll
-      for (int e = 0; e < kPart; ++e) w[i * kPart + e] = f.v[e];
+        for (int e = 0; e < kPart / 2; ++e) w[i * kPart / 2 + e] = pair_of(f.v[2 * e], f.v[2 * e + 1]);
+      }
     }
   }
 };
@@ -212,28 +269,33 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// The factors of a unit row: y_i = (x_i * pre) * inv.  Nearly every row is plain: its
-// sum of squares is well inside the 32-bit range and above eps^2.  For the others
-// the sum is taken again over x / max|x|.
+// The factors of a unit row.  Nearly every row is plain: its sum of squares is well inside
+// the 32-bit range and above eps^2, and y = x * rsqrt(sum).  For the others the sum is
+// taken again over x / top, top = max|x|: y = (x / top) * inv.
 struct UnitScale {
-  float pre, inv;
+  float inv;
+  bool scaled;   // inv belongs to x / top, else to x
   bool clamped;  // |x| <= eps: y = x / eps
 };
 __device__ __forceinline__ float least_square(float eps) { return fmaxf(1e-30f, 1.0001f * eps * eps); }
 __device__ __forceinline__ bool plain_square(float ss, float least) { return ss > least && ss < 1e37f; }
+// 1 / top as a product of two factors that both lie in the range, a power of two first.
+__device__ __forceinline__ float2 reciprocal_parts(float top) {
+  const float power = top > 1.f ? 5.421010862427522e-20f : 1.8446744073709552e19f;  // 2^-64, 2^64
+  return make_float2(power, 1.0f / (top * power));
+}
 // `ss` is that of x / top where top is positive and finite, else of x; a NaN stays one.
 __device__ __forceinline__ UnitScale unit_scale(float ss, float top, float eps) {
   const bool scaled = top > 0.f && top < INFINITY;
   const float norm = scaled ? top * sqrtf(ss) : sqrtf(ss);
   UnitScale u;
   if (norm == INFINITY && !scaled) {  // an infinity in the row: finite / inf = 0, inf / inf = NaN
-    u.pre = 1.0f;
     u.inv = 0.0f;
-    u.clamped = false;
+    u.scaled = u.clamped = false;
     return u;
   }
   u.clamped = norm <= eps;
-  u.pre = scaled && !u.clamped ? 1.0f / top : 1.0f;
+  u.scaled = scaled && !u.clamped;
   u.inv = u.clamped ? 1.0f / eps : 1.0f / sqrtf(ss);
   return u;
 }
@@ -246,7 +308,7 @@ __device__ __forceinline__ UnitScale unit_scale(float ss, float top, float eps) 
 // HBM-bound: what counts is bytes in flight.  Every thread copies its own packs of the
 // next rows into a ring in shared memory (cp.async) and reads back nothing but
 // what it copied itself, so the ring needs no barrier; the reductions and the store of a row run
-// under the loads of the next kStages - 1.
+// under the loads of the next.
 // ---------------------------------------------------------------------------
 constexpr int kWide = 128;  // threads of a team that is a CTA
 
@@ -274,19 +336,20 @@ enum Staging : int { kInPlace = 0, kPacks = 1, kWords = 2 };
 template <typename T, int E, int TEAM>
 constexpr Staging kStaging = sizeof(T) * E >= 4 ? kPacks : TEAM == 32 ? kWords : kInPlace;
 
-constexpr int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
-
-// Rows in the ring (one of them in use): as many as 200 KB of shared memory hold, 2 to 4.
-template <typename T, int E, int TEAM, int V, int TENSORS, int SM_THREADS>
-constexpr int kStages = clamp_int(200 * 1024 / (SM_THREADS * V * E * (int)sizeof(T) * TENSORS), 2, 4);
+// Rows in the ring, one of them in use.  More loads in flight did not help, they held the
+// stores up: 2, 3 and 4 stages took 159, 174 and 176 us for 2.4M x 96 fp16 unit rows (backward 222, 248, 249),
+// 69, 78 and 75 for a layer norm of 98k x 1024 bf16 rows.  A CTA that takes a row together, with barriers
+// between, is short of them forward: 199 us with 2, 156 with 3 or 4, for 24k x 4096 fp32 rows.
+template <int TEAM, int TENSORS>
+constexpr int kStages = TEAM > 32 && TENSORS == 1 ? 3 : 2;
 // Bytes of one tensor's part of a stage, all threads of the CTA.
 template <typename T, int E, int TEAM, int V>
 constexpr int kPartBytes = kStaging<T, E, TEAM> == kWords ? kCtaThreads<TEAM> / 32 * (64 * V + 16)
                                                           : kCtaThreads<TEAM> * V * E * (int)sizeof(T);
-template <typename T, int E, int TEAM, int V, int TENSORS, int SM_THREADS>
+template <typename T, int E, int TEAM, int V, int TENSORS>
 constexpr int kRingBytes = kStaging<T, E, TEAM> == kInPlace
                                ? 0
-                               : kStages<T, E, TEAM, V, TENSORS, SM_THREADS> * TENSORS * kPartBytes<T, E, TEAM, V>;
+                               : kStages<TEAM, TENSORS> * TENSORS * kPartBytes<T, E, TEAM, V>;
 
 // The column sums at the end of the backward kernel take the ring's place: element e
 // of a pack lies e * kSumPitch on, which meets no bank twice, written or read.
@@ -298,7 +361,7 @@ constexpr int kSumBytes = 2 * (kCtaThreads<TEAM> / TEAM) * E * kSumPitch<E, TEAM
 // What lies before the weights in the backward kernel's shared memory.
 template <typename T, int KIND, int E, int TEAM, int V>
 constexpr int kBackwardBytes = [] {
-  const int ring = kRingBytes<T, E, TEAM, V, 2, kBackwardThreads<KIND, E, TEAM, V>>;
+  const int ring = kRingBytes<T, E, TEAM, V, 2>;
   const int sums = KIND == kLayer ? kSumBytes<E, TEAM> : 0;
   return ring > sums ? ring : sums;
 }();
@@ -411,18 +474,18 @@ struct Ring {
   }
 };
 
-// The packed rows of a team: a unit (a warp, or the CTA of a wide team) takes t.chunk
-// consecutive ones and its teams take them in turn.
+// The packed rows of a CTA: t.chunk consecutive ones, which its teams take in turn, so that
+// what a CTA reads and writes at any moment lies together (295k x 768 bf16 rows packed out of 1024 x 512, backward:
+// 309 us; with consecutive rows for every warp 323 us).
 template <int TEAM>
 struct Turn {
-  static constexpr int kRows = TEAM >= 32 ? 1 : 32 / TEAM;  // rows of a unit at a time
-  int32_t begin, end, mine;  // of the unit; the team's place in its turn
+  static constexpr int kRows = kCtaThreads<TEAM> / TEAM;  // rows at a time
+  int32_t begin, end, mine;  // of the CTA; the team's place in its turn
   __device__ __forceinline__ Turn(const Rows& t) {
-    const int64_t unit = TEAM > 32 ? blockIdx.x : (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    const int64_t from = unit * t.chunk, used = t.used();
+    const int64_t from = (int64_t)blockIdx.x * t.chunk, used = t.used();
     begin = (int32_t)min(from, used);
     end = (int32_t)min(from + t.chunk, used);
-    mine = TEAM >= 32 ? 0 : (threadIdx.x & 31) / TEAM;
+    mine = threadIdx.x / TEAM;
   }
 };
 
@@ -431,7 +494,7 @@ __global__ void __launch_bounds__(kCtaThreads<TEAM>, kForwardThreads<E, TEAM, V>
 forward_rows_kernel(const T* __restrict__ tokens, const __grid_constant__ Rows t, Affine weight, Affine bias,
                     T* __restrict__ out, float* __restrict__ mean, float* __restrict__ rstd, float eps) {
   constexpr Staging kHow = kStaging<T, E, TEAM>;
-  constexpr int S = kHow != kInPlace ? kStages<T, E, TEAM, V, 1, kForwardThreads<E, TEAM, V>> : 1;
+  constexpr int S = kHow != kInPlace ? kStages<TEAM, 1> : 1;
   extern __shared__ __align__(16) char shared[];
   __shared__ float words[TEAM > 32 ? TEAM / 8 : 1];
   Team<TEAM> team(words);
@@ -457,7 +520,7 @@ forward_rows_kernel(const T* __restrict__ tokens, const __grid_constant__ Rows t
     for (int i = 0; i < S - 1; ++i) copy(i, turn.begin + turn.mine + i * R);
   }
   const int packs = (t.dim + E - 1) / E;
-  float* const after = reinterpret_cast<float*>(shared + kRingBytes<T, E, TEAM, V, 1, kForwardThreads<E, TEAM, V>>);
+  float* const after = reinterpret_cast<float*>(shared + kRingBytes<T, E, TEAM, V, 1>);
   const Wide<E> w{after, packs}, b{after + packs * E, packs};
   if constexpr (KIND == kLayer) {
     w.template fill<T>(weight, t.dim, 1.0f);
@@ -479,8 +542,10 @@ forward_rows_kernel(const T* __restrict__ tokens, const __grid_constant__ Rows t
       here.seek(t, row);
       x += here.from(t, row);
     }
-    float f[V][E];
-    float s = 0.f, ss = 0.f;
+    using X = Elem<E>;
+    constexpr int N = kElems<E>;
+    X f[V][N];  // zero where there is no element
+    X sum = splat<X>(0.f);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = (lane + TEAM * v) * E;
@@ -489,38 +554,39 @@ forward_rows_kernel(const T* __restrict__ tokens, const __grid_constant__ Rows t
         else expand(load_pack<T, E>(x + c), f[v]);
       } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) f[v][e] = 0.f;
+        for (int i = 0; i < N; ++i) f[v][i] = splat<X>(0.f);
       }
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (KIND == kLayer) s += f[v][e];
-        else ss += f[v][e] * f[v][e];
-      }
+      for (int i = 0; i < N; ++i) sum = KIND == kLayer ? add(f[v][i], sum) : fma(f[v][i], f[v][i], sum);
     }
     stage = stage == S - 1 ? 0 : stage + 1;
     if constexpr (KIND == kLayer) {
-      const float mu = team.sum(s) * per;
+      const float mu = team.sum(total(sum)) * per;
+      const X minus_mu = splat<X>(-mu);
+      sum = splat<X>(0.f);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const bool in = (lane + TEAM * v) * E < t.dim;
+        if ((lane + TEAM * v) * E < t.dim) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          f[v][e] = in ? f[v][e] - mu : 0.f;
-          ss += f[v][e] * f[v][e];
+          for (int i = 0; i < N; ++i) {
+            f[v][i] = add(f[v][i], minus_mu);
+            sum = fma(f[v][i], f[v][i], sum);
+          }
         }
       }
-      const float r = rsqrtf(team.sum(ss) * per + eps);
+      const float r = rsqrtf(team.sum(total(sum)) * per + eps);
       if (there) {
         T* const y = out + (int64_t)row * t.dim;
+        const X rr = splat<X>(r);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const int c = (lane + TEAM * v) * E;
           if (c < t.dim) {
-            float wv[E], bv[E];
+            X wv[N], bv[N];
             w.get(lane + TEAM * v, wv);
             b.get(lane + TEAM * v, bv);
 #pragma unroll
-            for (int e = 0; e < E; ++e) f[v][e] = f[v][e] * r * wv[e] + bv[e];
+            for (int i = 0; i < N; ++i) f[v][i] = fma(mul(f[v][i], rr), wv[i], bv[i]);
             store_pack<T, E>(y + c, compress<T, E>(f[v]));
           }
         }
@@ -530,7 +596,7 @@ forward_rows_kernel(const T* __restrict__ tokens, const __grid_constant__ Rows t
         }
       }
     } else {
-      ss = team.sum(ss);
+      const float ss = team.sum(total(sum));
       float inv = rsqrtf(ss);
       const bool plain = plain_square(ss, least) || !there;
       if (team.any(!plain)) {
@@ -538,32 +604,40 @@ forward_rows_kernel(const T* __restrict__ tokens, const __grid_constant__ Rows t
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
-          for (int e = 0; e < E; ++e) top = fmaxf(top, fabsf(f[v][e]));
+          for (int i = 0; i < N; ++i) top = fmaxf(top, most(f[v][i]));
         top = team.max(top);
         const bool scaled = top > 0.f && top < INFINITY;
-        float again = 0.f;
+        // x / top by its reciprocal, in two factors that do not leave the range
+        const float2 by = scaled ? reciprocal_parts(top) : make_float2(1.f, 1.f);
+        X again = splat<X>(0.f);
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
-          for (int e = 0; e < E; ++e) again += scaled ? (f[v][e] / top) * (f[v][e] / top) : 0.f;
-        again = team.sum(again);
+          for (int i = 0; i < N; ++i) {
+            const X d = mul(mul(f[v][i], splat<X>(by.x)), splat<X>(by.y));
+            again = fma(d, d, again);
+          }
+        const float ss2 = team.sum(total(again));
         if (!plain) {
-          const UnitScale u = unit_scale(scaled ? again : ss, top, eps);
+          const UnitScale u = unit_scale(scaled ? ss2 : ss, top, eps);
           inv = u.inv;
+          if (u.scaled) {
 #pragma unroll
-          for (int v = 0; v < V; ++v)
+            for (int v = 0; v < V; ++v)
 #pragma unroll
-            for (int e = 0; e < E; ++e) f[v][e] *= u.pre;
+              for (int i = 0; i < N; ++i) f[v][i] = mul(mul(f[v][i], splat<X>(by.x)), splat<X>(by.y));
+          }
         }
       }
       if (there) {
         T* const y = out + (int64_t)row * t.dim;
+        const X ii = splat<X>(inv);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const int c = (lane + TEAM * v) * E;
           if (c < t.dim) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) f[v][e] *= inv;
+            for (int i = 0; i < N; ++i) f[v][i] = mul(f[v][i], ii);
             store_pack<T, E>(y + c, compress<T, E>(f[v]));
           }
         }
@@ -603,7 +677,7 @@ backward_rows_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, c
                      T* __restrict__ grad_tokens, float* __restrict__ partial, float eps) {
   constexpr int kCta = kCtaThreads<TEAM>;
   constexpr Staging kHow = kStaging<T, E, TEAM>;
-  constexpr int S = kHow != kInPlace ? kStages<T, E, TEAM, V, 2, kBackwardThreads<KIND, E, TEAM, V>> : 1;
+  constexpr int S = kHow != kInPlace ? kStages<TEAM, 2> : 1;
   constexpr int kFixed = kBackwardBytes<T, KIND, E, TEAM, V>;
   extern __shared__ __align__(16) char shared[];
   __shared__ float words[TEAM > 32 ? TEAM / 8 : 1];
@@ -611,12 +685,12 @@ backward_rows_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, c
   const Ring<T, E, TEAM, V, 2> ring(shared);
   const int lane = threadIdx.x % TEAM;
   const float per = 1.0f / t.dim, least = least_square(eps);
-  float dw[KIND == kLayer ? V : 1][E], db[KIND == kLayer ? V : 1][E];
+  Elem<E> dw[KIND == kLayer ? V : 1][kElems<E>], db[KIND == kLayer ? V : 1][kElems<E>];
   if constexpr (KIND == kLayer) {
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
-      for (int e = 0; e < E; ++e) dw[v][e] = db[v][e] = 0.f;
+      for (int i = 0; i < kElems<E>; ++i) dw[v][i] = db[v][i] = splat<Elem<E>>(0.f);
   }
   const Turn<TEAM> turn(t);
   constexpr int R = Turn<TEAM>::kRows;
@@ -667,8 +741,10 @@ backward_rows_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, c
     }
     const T* const x_row = tokens + (kHow != kPacks && there ? here.from(t, row) : 0);
     const T* const g_row = grad + (there ? (int64_t)row * t.dim : 0);
+    using X = Elem<E>;
+    constexpr int N = kElems<E>;
     // pack v of the row and of its gradient
-    const auto packs_of = [&](int v, float (&x)[E], float (&g)[E]) {
+    const auto packs_of = [&](int v, X (&x)[N], X (&g)[N]) {
       if constexpr (kHow != kInPlace) {
         expand(ring.pack(stage, 0, v, x_row), x);
         expand(ring.pack(stage, 1, v, g_row), g);
@@ -681,99 +757,106 @@ backward_rows_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, c
     T* const dx = grad_tokens + (there ? here.slot(t, row) * t.dim : 0);
     const bool store = grad_tokens && there;
     if constexpr (KIND == kLayer) {
-      float su = 0.f, suh = 0.f;
+      X su = splat<X>(0.f), suh = su;
+      const X minus_mu = splat<X>(-mu), rr = splat<X>(r);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         if (there && (lane + TEAM * v) * E < t.dim) {
-          float x[E], g[E], wv[E];
+          X x[N], g[N], wv[N];
           packs_of(v, x, g);
           w.get(lane + TEAM * v, wv);
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const float h = (x[e] - mu) * r, u = g[e] * wv[e];
-            su += u;
-            suh += u * h;
-            dw[v][e] += g[e] * h;
-            db[v][e] += g[e];
+          for (int i = 0; i < N; ++i) {
+            const X h = mul(add(x[i], minus_mu), rr), u = mul(g[i], wv[i]);
+            su = add(u, su);
+            suh = fma(u, h, suh);
+            dw[v][i] = fma(g[i], h, dw[v][i]);
+            db[v][i] = add(g[i], db[v][i]);
           }
         }
       }
-      const float2 both = team.sums(su, suh);
+      const float2 both = team.sums(total(su), total(suh));
       // dx = r (u - mean(u) - h mean(u h))
-      const float minus_u = -r * (both.x * per), minus_h = -r * (both.y * per);
+      const X minus_u = splat<X>(-r * (both.x * per)), minus_h = splat<X>(-r * (both.y * per));
       asm volatile("" ::: "memory");  // read the packs again instead of keeping them
       if (store) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const int c = (lane + TEAM * v) * E;
           if (c < t.dim) {
-            float x[E], g[E], wv[E];
+            X x[N], g[N], wv[N];
             packs_of(v, x, g);
             w.get(lane + TEAM * v, wv);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-              const float h = (x[e] - mu) * r;
-              x[e] = g[e] * wv[e] * r + (h * minus_h + minus_u);
+            for (int i = 0; i < N; ++i) {
+              const X h = mul(add(x[i], minus_mu), rr);
+              x[i] = fma(mul(g[i], wv[i]), rr, fma(h, minus_h, minus_u));
             }
             store_pack<T, E>(dx + c, compress<T, E>(x));
           }
         }
       }
     } else {
-      float x[V][E], g[V][E];
-      float ss = 0.f, xg = 0.f;
+      X x[V][N], g[V][N];
+      X squares = splat<X>(0.f), products = squares;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         if (there && (lane + TEAM * v) * E < t.dim) {
           packs_of(v, x[v], g[v]);
         } else {
 #pragma unroll
-          for (int e = 0; e < E; ++e) x[v][e] = g[v][e] = 0.f;
+          for (int i = 0; i < N; ++i) x[v][i] = g[v][i] = splat<X>(0.f);
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          ss += x[v][e] * x[v][e];
-          xg += x[v][e] * g[v][e];
+        for (int i = 0; i < N; ++i) {
+          squares = fma(x[v][i], x[v][i], squares);
+          products = fma(x[v][i], g[v][i], products);
         }
       }
-      const float2 both = team.sums(ss, xg);
-      ss = both.x;
-      xg = both.y;
-      float inv = rsqrtf(ss), pre = 1.0f, along = xg * inv;  // along: y . g
+      const float2 both = team.sums(total(squares), total(products));
+      const float ss = both.x, xg = both.y;
+      float inv = rsqrtf(ss), scale = inv, along = xg * inv;  // along: y . g; dx = (g - y along) * scale
       const bool plain = plain_square(ss, least) || !there;
       if (team.any(!plain)) {
         float top = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
-          for (int e = 0; e < E; ++e) top = fmaxf(top, fabsf(x[v][e]));
+          for (int i = 0; i < N; ++i) top = fmaxf(top, most(x[v][i]));
         top = team.max(top);
         const bool scaled = top > 0.f && top < INFINITY;
-        float ss2 = 0.f, xg2 = 0.f;
+        const float2 by = scaled ? reciprocal_parts(top) : make_float2(1.f, 1.f);
+        squares = products = splat<X>(0.f);
 #pragma unroll
         for (int v = 0; v < V; ++v)
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const float xv = scaled ? x[v][e] / top : 0.f;
-            ss2 += xv * xv;
-            xg2 += xv * g[v][e];
+          for (int i = 0; i < N; ++i) {
+            const X d = mul(mul(x[v][i], splat<X>(by.x)), splat<X>(by.y));
+            squares = fma(d, d, squares);
+            products = fma(d, g[v][i], products);
           }
-        const float2 again = team.sums(ss2, xg2);
+        const float2 again = team.sums(total(squares), total(products));
         if (!plain) {
           const UnitScale u = unit_scale(scaled ? again.x : ss, top, eps);
-          inv = u.inv;
-          pre = u.pre;
+          inv = scale = u.inv;
           along = u.clamped ? 0.0f : (scaled ? again.y : xg) * inv;
+          if (u.scaled) {
+            scale = inv * by.x * by.y;
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+#pragma unroll
+              for (int i = 0; i < N; ++i) x[v][i] = mul(mul(x[v][i], splat<X>(by.x)), splat<X>(by.y));
+          }
         }
       }
       if (store) {
-        const float scale = inv * pre, minus = -along * scale;
+        const X ii = splat<X>(inv), kk = splat<X>(scale), minus = splat<X>(-along);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const int c = (lane + TEAM * v) * E;
           if (c < t.dim) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[v][e] = g[v][e] * scale + x[v][e] * pre * inv * minus;
+            for (int i = 0; i < N; ++i) x[v][i] = mul(fma(mul(x[v][i], ii), minus, g[v][i]), kk);
             store_pack<T, E>(dx + c, compress<T, E>(x[v]));
           }
         }
@@ -789,10 +872,11 @@ backward_rows_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, c
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       __syncthreads();
+      const Pack<float, E> pw = unpacked<E>(dw[v]), pb = unpacked<E>(db[v]);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        acc[0][threadIdx.x / TEAM][e * kPitch + lane] = dw[v][e];
-        acc[1][threadIdx.x / TEAM][e * kPitch + lane] = db[v][e];
+        acc[0][threadIdx.x / TEAM][e * kPitch + lane] = pw.v[e];
+        acc[1][threadIdx.x / TEAM][e * kPitch + lane] = pb.v[e];
       }
       __syncthreads();
       for (int i = threadIdx.x; i < 2 * TEAM * E; i += kCta) {
@@ -843,7 +927,7 @@ forward_wide_kernel(const T* __restrict__ tokens, Rows t, Affine weight, Affine 
   const Turn<32> turn(t);
   Walker here;
   if (turn.begin < turn.end) here.find(t, turn.begin);
-  for (int32_t row = turn.begin; row < turn.end; ++row) {
+  for (int32_t row = turn.begin + turn.mine; row < turn.end; row += Turn<32>::kRows) {
     here.seek(t, row);
     const T* x = tokens + here.from(t, row);
     T* y = out + (int64_t)row * t.dim;
@@ -875,20 +959,24 @@ forward_wide_kernel(const T* __restrict__ tokens, Rows t, Affine weight, Affine 
         top = fmaxf(top, fabsf(v));
       }
       ss = warp_sum(ss);
-      UnitScale u{1.0f, rsqrtf(ss), false};
+      float inv = rsqrtf(ss);
+      float2 by = make_float2(1.f, 1.f);
       if (!plain_square(ss, least_square(eps))) {
         top = warp_max(top);
         if (top > 0.f && top < INFINITY) {
+          by = reciprocal_parts(top);
           ss = 0.f;
           for (int c = lane; c < t.dim; c += 32) {
-            const float v = widen(x[c]) / top;
+            const float v = widen(x[c]) * by.x * by.y;
             ss += v * v;
           }
           ss = warp_sum(ss);
         }
-        u = unit_scale(ss, top, eps);
+        const UnitScale u = unit_scale(ss, top, eps);
+        inv = u.inv;
+        if (!u.scaled) by = make_float2(1.f, 1.f);
       }
-      for (int c = lane; c < t.dim; c += 32) y[c] = narrow<T>(widen(x[c]) * u.pre * u.inv);
+      for (int c = lane; c < t.dim; c += 32) y[c] = narrow<T>(widen(x[c]) * by.x * by.y * inv);
     }
   }
 }
@@ -906,7 +994,7 @@ backward_wide_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, R
     zero_padding<T, 1>(t, grad_tokens, (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5),
                        (int64_t)gridDim.x * (kThreads / 32), lane, 32);
   if (turn.begin < turn.end) here.find(t, turn.begin);
-  for (int32_t row = turn.begin; row < turn.end; ++row) {
+  for (int32_t row = turn.begin + turn.mine; row < turn.end; row += Turn<32>::kRows) {
     here.seek(t, row);
     const T* x = tokens + here.from(t, row);
     const T* g = grad + (int64_t)row * t.dim;
@@ -935,25 +1023,29 @@ backward_wide_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, R
       }
       ss = warp_sum(ss);
       xg = warp_sum(xg);
-      UnitScale u{1.0f, rsqrtf(ss), false};
+      float inv = rsqrtf(ss), along = xg * inv;  // along: y . g
+      float2 by = make_float2(1.f, 1.f);
       if (!plain_square(ss, least_square(eps))) {
         top = warp_max(top);
         if (top > 0.f && top < INFINITY) {
+          by = reciprocal_parts(top);
           ss = xg = 0.f;
           for (int c = lane; c < t.dim; c += 32) {
-            const float v = widen(x[c]) / top;
+            const float v = widen(x[c]) * by.x * by.y;
             ss += v * v;
             xg += v * widen(g[c]);
           }
           ss = warp_sum(ss);
           xg = warp_sum(xg);
         }
-        u = unit_scale(ss, top, eps);
+        const UnitScale u = unit_scale(ss, top, eps);
+        inv = u.inv;
+        along = u.clamped ? 0.0f : xg * inv;
+        if (!u.scaled) by = make_float2(1.f, 1.f);
       }
-      const float along = u.clamped ? 0.0f : xg * u.inv;  // y . g
       for (int c = lane; c < t.dim; c += 32) {
-        const float h = widen(x[c]) * u.pre * u.inv;
-        dx[c] = narrow<T>((widen(g[c]) - h * along) * u.inv * u.pre);
+        const float h = widen(x[c]) * by.x * by.y * inv;
+        dx[c] = narrow<T>((widen(g[c]) - h * along) * inv * by.x * by.y);
       }
     }
   }

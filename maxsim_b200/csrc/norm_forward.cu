@@ -24,7 +24,7 @@ struct Forward {
   template <typename T, int KIND, int E, int TEAM, int V>
   int rows() const {
     constexpr int threads = norm::kCtaThreads<TEAM>, per_sm = norm::kForwardThreads<E, TEAM, V>;
-    constexpr int ring = norm::kRingBytes<T, E, TEAM, V, 1, per_sm>;
+    constexpr int ring = norm::kRingBytes<T, E, TEAM, V, 1>;
     auto kern = norm::forward_rows_kernel<T, KIND, E, TEAM, V>;
     static std::atomic<unsigned char> configured[kMaxDevices];
     constexpr int most = ring + (KIND == norm::kLayer ? 2 * norm::Wide<E>::bytes(TEAM * V * E) : 0);

@@ -18,8 +18,8 @@ constexpr int64_t kMaxRows = (1ll << 31) - 4096;  // 32-bit row counters run a f
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// How the packed rows are split over a grid: every unit (a warp, or the CTA of a
-// wide team) gets the same number of consecutive rows.
+// How the packed rows are split over a grid: every CTA gets the same number of
+// consecutive rows, whole turns of its teams.
 struct Split {
   unsigned grid;
   int32_t chunk;
@@ -30,10 +30,10 @@ struct Split {
 };
 template <int THREADS, int TEAM>
 Split share_rows(int64_t rows, int ctas_per_sm) {
-  constexpr int units = TEAM > 32 ? 1 : THREADS / 32, together = TEAM >= 32 ? 1 : 32 / TEAM;
-  const int64_t most = (int64_t)sm_count() * ctas_per_sm * units;
+  constexpr int together = THREADS / TEAM;
+  const int64_t most = (int64_t)sm_count() * ctas_per_sm;
   const int64_t chunk = ceil_div(ceil_div(rows, most), together) * together;
-  return {(unsigned)ceil_div(ceil_div(rows, chunk), units), (int32_t)chunk};
+  return {(unsigned)ceil_div(rows, chunk), (int32_t)chunk};
 }
 
 // The team a row gets.  Few threads with many packs cost fewer instructions a row (the
