@@ -301,12 +301,12 @@ __device__ __forceinline__ UnitScale unit_scale(float ss, float top, float eps) 
 }
 
 // ---------------------------------------------------------------------------
-// Rows shared by a team of TEAM threads (8, 16 or 32 lanes of a warp, or a CTA of
+// Rows shared by a team of TEAM threads (2 to 32 lanes of a warp, or a CTA of
 // 128); a thread has V packs of E elements of a row.  Every element is read once and
 // written once.
 //
-// HBM-bound: what counts is bytes in flight.  Every thread copies its own packs of the
-// next rows into a ring in shared memory (cp.async) and reads back nothing but
+// HBM-bound for rows of wide packs: 5.3 to 6.2 TB/s of a copy's 6.5.  Every thread copies its own packs
+// of the next row into a ring in shared memory (cp.async) and reads back nothing but
 // what it copied itself, so the ring needs no barrier; the reductions and the store of a row run
 // under the loads of the next.
 // ---------------------------------------------------------------------------
@@ -315,10 +315,12 @@ constexpr int kWide = 128;  // threads of a team that is a CTA
 template <int TEAM>
 constexpr int kCtaThreads = TEAM > 32 ? TEAM : kThreads;
 
-// Threads an SM is to hold at once: what the registers are cut to.  With wide packs the
-// ring keeps enough bytes in flight for fewer threads with more registers (layer norm of 130k x 768 bf16 rows,
-// 512 and 768 threads: 71.8 and 76.4 us; with teams of a CTA and four packs, which wait at barriers, 24k x
-// 4096: 136 and 106 us); narrow packs are short of instructions and want the threads (200k x 500: 198 and 172).
+// Threads an SM is to hold at once: what the registers are cut to.  More threads are more
+// rows in flight, which past some point only hold the stores up.  Measured, 10^8 elements, us: layer norm
+// forward, 98k x 1024 bf16, 256 / 512 / 768 threads: 91 / 69 / 80; 781k x 128, 512 / 768 / 1024: 79 / 69 / 80; teams of a
+// CTA with four packs, which wait at barriers, 24k x 4096: 110 / - / 103.  Rows without wide packs are short of
+// instructions instead and take all they get.  Layer norm backward, 781k x 128 and 300k x 333 bf16, 512 / 768: 128 / 117
+// and 293 / 258; unit rows backward, 391k x 384 bf16, 256 / 512 / 768: 108 / 103 / 115.
 template <int E, int TEAM, int V>
 constexpr int kForwardThreads = V * E <= 8                               ? 1024
                                 : E < 4                                  ? (V * E <= 16 ? 1024 : 768)
@@ -326,8 +328,9 @@ constexpr int kForwardThreads = V * E <= 8                               ? 1024
                                 : E == 8 && TEAM == kWide                ? 768
                                                                          : 512;
 template <int KIND, int E, int TEAM, int V>
-constexpr int kBackwardThreads =
-    KIND == kUnit ? (V * E <= 8 ? 1024 : V * E <= 16 ? 768 : 512) : V * E <= 8 ? 768 : 512;
+constexpr int kBackwardThreads = KIND == kUnit ? (V * E <= 8 ? 1024 : V * E <= 16 ? 768 : 512)
+                                 : V * E <= 8 || (V * E <= 16 && TEAM <= 32) ? 768
+                                                                             : 512;
 
 // How a row's elements get into the ring: a thread's own packs of 16 or 4 bytes; for rows of
 // 16-bit elements that start and end anywhere, the 4-byte words around them, which

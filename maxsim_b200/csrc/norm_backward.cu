@@ -35,9 +35,13 @@ struct Backward {
     constexpr int most = fixed + (KIND == norm::kLayer ? norm::Wide<E>::bytes(TEAM * V * E) : 0);
     static_assert(most <= 227 * 1024, "shared memory of a CTA");
     if (int rc = ensure_smem(kern, most, configured)) return rc;
-    Split split = share_rows<threads, TEAM>(std::max(t.rows, 1), per_sm / threads);
+    // Unit rows that fill two packs of every lane keep enough in flight with two CTAs on an SM instead
+    // of three (781k x 128 bf16 93 and 105 us); rows that fill them in part do not (1042k x 96: 108 and 97).
+    const bool full = KIND == norm::kUnit && V * E == 16 && t.dim == TEAM * V * E;
+    const int ctas = full ? std::min(512, per_sm) / threads : per_sm / threads;
+    Split split = share_rows<threads, TEAM>(std::max(t.rows, 1), ctas);
     if (t.offsets) {  // few rows in much padding: as many CTAs as its zeros keep busy
-      const int64_t most_ctas = (int64_t)sm_count() * (per_sm / threads);
+      const int64_t most_ctas = (int64_t)sm_count() * ctas;
       split.grid = (unsigned)std::max<int64_t>(split.grid, std::min(most_ctas, ceil_div((int64_t)t.n_segments * t.L_max, 64)));
     }
     slabs = (int)split.grid;
