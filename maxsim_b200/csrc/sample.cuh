@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 sample_rows_kernel(const __grid_constant__ Args A) {
   using S = Shared<THREADS>;
   constexpr int kBins = S::kBins, kListed = S::kListed;
-  extern __shared__ float cache[];
+  extern __shared__ __align__(16) float cache[];
   __shared__ S sh;
   Block<THREADS> block{sh};
   const int64_t row = blockIdx.x;
@@ -340,7 +340,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
     }
     return;
   }
-  const double inv_T = 1.0 / T, per_bit = inv_T * 1.4426950408889634;
+  const double inv_T = fmin(1.0 / T, 1e300), per_bit = inv_T * 1.4426950408889634;
   // candidates are the scores from `first` on (false for NaN and -inf)
   const float first = (double)least - (double)best > -699.0 * T
                           ? least

@@ -47,7 +47,7 @@ def test_filters(C, kw):
     check(s, u, min(C, 9), temperature=0.3, **kw)
 
 
-@pytest.mark.parametrize("T", [1e-3, 0.05, 1.0, 30.0, INF])
+@pytest.mark.parametrize("T", [1e-310, 1e-3, 0.05, 1.0, 30.0, 1e300, INF])
 def test_temperatures(T):
     s, u = scores_of(6, 300, 1)
     check(s, u, 20, temperature=T, top_p=0.9)
@@ -159,6 +159,11 @@ def test_scores_at_every_scale():
             check(s, u, 20, temperature=T, **kw)
     check(torch.tensor([[7.0, 0.0, 1e-30, -1e-30, 3.5]]), torch.tensor([[0.5, 0.6, 0.7, 0.8, 0.9]]), 5, temperature=0.01)
     check(torch.zeros(1, 400), torch.rand(1, 400, generator=g), 9, min_p=1.0)
+    infinite = s.clone()
+    infinite[:, ::5] = INF
+    for T in (1e-310, 1.0, INF):
+        for kw in (dict(), dict(top_k=300), dict(top_p=0.6), dict(min_p=0.5)):
+            check(infinite, u, 20, temperature=T, **kw)
 
 
 def test_uniforms_below_the_normal_range():
