@@ -195,6 +195,15 @@ MAXSIM_API int maxsim_b200_norm_rows(int norm, const void* tokens, int64_t segme
                                      float* mean, float* rstd, int64_t n_segments,
                                      int64_t L_max, int64_t dim, int64_t packed_rows,
                                      double eps, int dtype, int weight_dtype, void* stream);
+/* norm_rows of a padded batch in one call: writes offsets [n_segments + 1] as
+ * maxsim_b200_offsets_from_lengths does from lengths [n_segments], then packs. */
+MAXSIM_API int maxsim_b200_pack_norm_rows(int norm, const void* padded, int64_t segment_stride,
+                                          int64_t row_stride, const int32_t* lengths,
+                                          int32_t* offsets, const void* weight,
+                                          const void* bias, void* packed, float* mean,
+                                          float* rstd, int64_t n_segments, int64_t L_max,
+                                          int64_t dim, int64_t packed_rows, double eps,
+                                          int dtype, int weight_dtype, void* stream);
 MAXSIM_API int64_t maxsim_b200_norm_rows_workspace(int64_t n_segments, int64_t L_max, int64_t dim);
 MAXSIM_API int maxsim_b200_norm_rows_backward(int norm, const void* grad, const void* tokens,
                                               int64_t segment_stride, int64_t row_stride,

@@ -52,6 +52,7 @@ _SIGNATURES = {
     "maxsim_b200_sample_rows": (c_int, [_P, _I64, _P, _I64, _I64, _I64, _I64, _F64, _P, _I64, _P, _F64, _P, _F64, _P]
                                 + [_P] * 3),
     "maxsim_b200_norm_rows": (c_int, [c_int, _P, _I64, _I64] + [_P] * 6 + [_I64] * 4 + [_F64, c_int, c_int, _P]),
+    "maxsim_b200_pack_norm_rows": (c_int, [c_int, _P, _I64, _I64] + [_P] * 7 + [_I64] * 4 + [_F64, c_int, c_int, _P]),
     "maxsim_b200_norm_rows_workspace": (c_int64, [_I64] * 3),
     "maxsim_b200_norm_rows_backward": (c_int, [c_int, _P, _P, _I64, _I64] + [_P] * 8 + [_I64] * 5
                                        + [_F64, c_int, c_int, _P]),
@@ -304,24 +305,28 @@ def sample_rows(scores: torch.Tensor, uniforms: torch.Tensor, n: int, temperatur
 NORM_LAYER, NORM_UNIT = 0, 1
 
 
-def norm_rows(kind: int, tokens: torch.Tensor, call, offsets, weight, bias, eps: float, out_shape, want_stats: bool):
+def norm_rows(kind: int, tokens: torch.Tensor, call, offsets, weight, bias, eps: float, out_shape, want_stats: bool,
+              lengths=None):
     """Normalise the rows of ``tokens``.  ``call`` is ``(stride of a segment,
     stride of a row, n_segments, L_max, dim, packed_rows)``, the strides in
     elements; the last dimension is contiguous.  With ``offsets [n_segments + 1]``
     int32 the rows that count are written back to back.  Returns ``(out, stats)``:
     ``out`` of ``packed_rows`` rows in ``out_shape``; the statistics ``[2, packed_rows]``
     fp32 (means, then reciprocal standard deviations) are None unless asked for
-    (layer norm only)."""
+    (layer norm only).  With ``lengths [n_segments]`` int32 the offsets are written
+    first."""
     segment_stride, row_stride, n, L, dim, packed_rows = call
+    lib = load_library()
     out = tokens.new_empty(out_shape)
     stats = tokens.new_empty((2, packed_rows), dtype=torch.float32) if want_stats else None
     at = stats.data_ptr() if want_stats else 0
+    where = () if lengths is None else (lengths.data_ptr(),)
+    fn = lib.maxsim_b200_norm_rows if lengths is None else lib.maxsim_b200_pack_norm_rows
     with _on_device(tokens.device):
-        rc = load_library().maxsim_b200_norm_rows(
-            kind, tokens.data_ptr(), segment_stride, row_stride, 0 if offsets is None else offsets.data_ptr(),
-            0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(), out.data_ptr(),
-            at, at + 4 * packed_rows if at else 0, n, L, dim, packed_rows, eps,
-            _code(tokens), 0 if weight is None else _code(weight), _stream_ptr())
+        rc = fn(kind, tokens.data_ptr(), segment_stride, row_stride, *where,
+                0 if offsets is None else offsets.data_ptr(), 0 if weight is None else weight.data_ptr(),
+                0 if bias is None else bias.data_ptr(), out.data_ptr(), at, at + 4 * packed_rows if at else 0,
+                n, L, dim, packed_rows, eps, _code(tokens), 0 if weight is None else _code(weight), _stream_ptr())
     _check(rc, "maxsim_b200_norm_rows")
     return out, stats
 

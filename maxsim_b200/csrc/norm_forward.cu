@@ -72,4 +72,18 @@ int maxsim_b200_norm_rows(int kind, const void* tokens, int64_t segment_stride, 
                                      static_cast<cudaStream_t>(stream)});
 }
 
+int maxsim_b200_pack_norm_rows(int kind, const void* padded, int64_t segment_stride, int64_t row_stride,
+                               const int32_t* lengths, int32_t* offsets, const void* weight, const void* bias,
+                               void* packed, float* mean, float* rstd, int64_t n_segments, int64_t L_max,
+                               int64_t dim, int64_t packed_rows, double eps, int dtype, int weight_dtype,
+                               void* stream) {
+  if (!offsets) return fail(MAXSIM_EINVAL, "null pointer argument");
+  norm::Rows t;  // refuse before anything is written
+  if (int rc = check_rows(kind, n_segments, L_max, dim, packed_rows, segment_stride, row_stride, offsets, eps, &t))
+    return rc;
+  if (int rc = maxsim_b200_offsets_from_lengths(lengths, n_segments, L_max, offsets, nullptr, stream)) return rc;
+  return maxsim_b200_norm_rows(kind, padded, segment_stride, row_stride, offsets, weight, bias, packed, mean, rstd,
+                               n_segments, L_max, dim, packed_rows, eps, dtype, weight_dtype, stream);
+}
+
 }  // extern "C"

@@ -46,13 +46,15 @@ def _rows(tokens: torch.Tensor):
 
 class _NormFn(torch.autograd.Function):
     """``call`` is ``(kind, source rows, their strides and sizes, offsets, eps,
-    shape of the result)``.  The statistics of a layer norm are saved for the
-    backward pass; a unit row's length is taken again from the row."""
+    shape of the result, lengths the offsets are to be written from or None)``.  The
+    statistics of a layer norm are saved for the backward pass; a unit row's length
+    is taken again from the row."""
 
     @staticmethod
     def forward(ctx, tokens, weight, bias, call):
-        kind, src, rows, offsets, eps, out_shape = call
-        out, stats = _ops.norm_rows(kind, src, rows, offsets, weight, bias, eps, out_shape, kind == _ops.NORM_LAYER)
+        kind, src, rows, offsets, eps, out_shape, lengths = call
+        out, stats = _ops.norm_rows(kind, src, rows, offsets, weight, bias, eps, out_shape, kind == _ops.NORM_LAYER,
+                                    lengths)
         ctx.save_for_backward(src, weight, stats, offsets)
         ctx.call = (kind, rows, eps, tokens.shape)
         return out
@@ -75,7 +77,7 @@ def _backward(ctx, grad):
 _backward_once = once_differentiable(_backward)
 
 
-def _apply(kind, tokens, weight, bias, offsets, total, eps):
+def _apply(kind, tokens, weight, bias, offsets, total, eps, lengths=None):
     """``offsets`` None: rows in, rows out."""
     if offsets is None:
         src, rows = _rows(tokens)
@@ -88,8 +90,8 @@ def _apply(kind, tokens, weight, bias, offsets, total, eps):
     bias = bias if bias is None else bias.contiguous()
     if torch.is_grad_enabled() and (tokens.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
-        return _NormFn.apply(tokens, weight, bias, (kind, src, rows, offsets, eps, out_shape))
-    return _ops.norm_rows(kind, src, rows, offsets, weight, bias, eps, out_shape, False)[0]
+        return _NormFn.apply(tokens, weight, bias, (kind, src, rows, offsets, eps, out_shape, lengths))
+    return _ops.norm_rows(kind, src, rows, offsets, weight, bias, eps, out_shape, False, lengths)[0]
 
 
 def _check(name: str, tokens, weight, bias, eps) -> None:
@@ -124,6 +126,11 @@ def _packed(kind, padded, lengths, weight, bias, eps, total_tokens):
     if padded.dim() != 3:
         raise ValueError(f"padded must be 3-D [N, L_max, D]; got shape {tuple(padded.shape)}")
     _check("padded", padded, weight, bias, eps)
+    if (total_tokens is not None and lengths.dtype == torch.int32 and lengths.device == padded.device
+            and lengths.dim() == 1 and lengths.shape[0] == padded.shape[0] and lengths.is_contiguous()):
+        # nothing to look at on the host: offsets and rows in one call of the library
+        offsets = lengths.new_empty((lengths.shape[0] + 1,))
+        return _apply(kind, padded, weight, bias, offsets, int(total_tokens), float(eps), lengths), offsets
     offsets, total = packed_offsets(padded, lengths, total_tokens)
     return _apply(kind, padded, weight, bias, offsets, total, float(eps)), offsets
 

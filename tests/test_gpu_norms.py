@@ -465,6 +465,31 @@ def test_a_short_total_drops_rows_and_writes_no_others():
     check_layer(kept, w, None, g, y, (torch.cat([dx[0], dx[1, :3], dx[2, :2]]), dw, None))
 
 
+@pytest.mark.parametrize("lens,total", [([3, 0, 7, 5], 15), ([9, -2, 3, 1], 11), ([1, 2, 3, 4], 12), ([7] * 4, 20),
+                                        ([0, 0, 0, 0], 0), ([], 0)])
+def test_both_ways_of_writing_the_offsets(lens, total):
+    """int32 lengths on the device with a total take one call of the library, int64
+    ones two: lengths outside [0, L_max] and totals off the sum give the same."""
+    L = 7
+    x = rows_of((len(lens), L, 40), torch.float16, 0).requires_grad_(True)
+    w = rows_of((40,), torch.float32, 1).requires_grad_(True)
+    g = rows_of((total, 40), torch.float16, 2)
+    used = min(total, sum(min(max(n, 0), L) for n in lens))
+    got = []
+    for dtype in (torch.int32, torch.int64):
+        y, off = maxsim.pack_layer_norm(x, torch.tensor(lens, dtype=dtype, device=DEV), w, w, total_tokens=total)
+        assert y.shape == (total, 40)
+        dx, dw = torch.autograd.grad(y, (x, w), g)
+        u, off_u = maxsim.pack_unit_norm(x.detach(), torch.tensor(lens, dtype=dtype, device=DEV), total_tokens=total)
+        got.append((y.detach()[:used], off, dx, dw, u[:used], off_u))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    valid = torch.arange(L)[None, :] < torch.tensor(lens, dtype=torch.int64).reshape(-1, 1)
+    kept = x.detach()[valid.to(DEV)][:used]
+    if used:
+        check_layer(kept, w, w, None, got[0][0], None)
+
+
 @pytest.mark.parametrize("dim,dtype", [(768, torch.bfloat16), (333, torch.float32), (5000, torch.float16)])
 def test_equal_calls_give_equal_bits(dim, dtype):
     x = rows_of((3000, dim), dtype, 0).requires_grad_(True)

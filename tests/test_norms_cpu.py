@@ -173,6 +173,10 @@ def test_c_entries_refuse_without_touching_a_device():
     odd = lambda at, dt: lib.maxsim_b200_norm_rows(0, at, 32, 8, 0, 0, 0, 16, 0, 0, 1, 4, 8, 4, 1e-5, dt, dt, 0)  # noqa: E731
     assert odd(18, 0) == -1 and "element size" in error() and odd(17, 1) == -1
     assert norm(dt=0, wdt=1) == -2 and norm(dt=7) == -1 and "dtype" in error()
+    pack = lambda off=8, dim=8, n=1: lib.maxsim_b200_pack_norm_rows(  # noqa: E731
+        0, 16, 32, dim, 0, off, 0, 0, 16, 0, 0, n, 4, dim, 4, 1e-5, 0, 0, 0)
+    assert pack(off=0) == -1 and pack() == -1 and "null" in error()  # no lengths
+    assert pack(dim=0) == -1 and pack(n=2 ** 40) == -2
     assert lib.maxsim_b200_norm_rows_workspace(0, 4, 8) == 0
     back = lambda dw=0, ws=0, nbytes=0, kind=0: lib.maxsim_b200_norm_rows_backward(  # noqa: E731
         kind, 8, 8, 32, 8, 0, 0, 8, 8, 0, dw, 0, ws, nbytes, 1, 4, 8, 4, 1e-5, 0, 0, 0)
