@@ -23,6 +23,7 @@
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <string.h>
 
 #include "async.cuh"
 
@@ -154,6 +155,39 @@ struct Or {
   __device__ __forceinline__ int operator()(int a, int b) const { return a | b; }
 };
 
+// The CTAs of a cluster and each other's shared memory.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_ctas() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+// What every thread of the cluster wrote to any of its CTAs before is seen by all of them afterwards.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// The address of a CTA's own shared variable in the CTA of that rank.
+__device__ __forceinline__ uint32_t at_rank(const void* mine, uint32_t rank) {
+  uint32_t there;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
+  return there;
+}
+__device__ __forceinline__ void store_at(uint32_t there, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(there), "r"(v) : "memory");
+}
+__device__ __forceinline__ void store_at(uint32_t there, unsigned long long v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(there), "l"(v) : "memory");
+}
+__device__ __forceinline__ uint2 load_pair_at(uint32_t there) {
+  uint2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(there) : "memory");
+  return v;
+}
+
 // A CTA per row.  The row's scores are kept in shared memory (kCached, up to
 // kMostCached columns) or read again from memory for each pass; with the race
 // they are overwritten by its values.
@@ -170,12 +204,19 @@ struct Or {
 // with the arithmetic's error taken off, whose n-th largest leaves out everything
 // that cannot be among the n best; and in 64 bits for the few that are left.
 //
+// Few long rows get a cluster of CTAs each (kCluster): a CTA takes a slice of the row,
+// reductions go on through the other CTAs' shared memory, every CTA adds up all the
+// histograms, and every CTA comes to the same cut.  The candidates left for the 64-bit race
+// go to the cluster's first CTA.  All branches around a cluster's barrier hang on values that are the
+// same in all its CTAs.
+//
 // What bounds it: instructions and latency, not memory.  A row is read once, but
 // every element then takes an exponential, two logarithms and a histogram step, and a
 // row goes through some twenty barriers.
 constexpr int kRaced = 2048;         // candidates of a row that are raced in 64 bits (a power of two)
 constexpr int kFew = 384;            // kept candidates that go to the 64-bit race without the 32-bit one
-constexpr int kMostCached = 40960;   // columns of a row in shared memory
+constexpr int kMostCached = 40960;   // columns of a row (or of a CTA's slice) in shared memory
+constexpr int kMostCtas = 16;        // of a cluster
 
 template <int THREADS>
 struct Shared {
@@ -192,17 +233,21 @@ struct Shared {
   };
   int32_t list[kRaced];
   unsigned long long words[2][5][THREADS / 32];
+  unsigned long long ranks[2][5][kMostCtas];  // what the CTAs of a cluster reduced, by rank
+  float all_score[kListed];                   // members of all CTAs
+  int32_t all_index[kListed];
   unsigned long long found_above;
   float found_score;
   int32_t found_bin, found_index, members;
 };
 
-template <int THREADS>
+template <int THREADS, bool kCluster>
 struct Block {
   Shared<THREADS>& sh;
-  int half = 0;
+  uint32_t rank, ctas;
+  int half = 0, ranks_half = 0;
 
-  // Every thread gets the results over all threads; up to five values at once.  One
+  // Every thread gets the results over all threads (of all CTAs); up to five values at once.  One
   // barrier: the next call uses the other words.
   template <typename V, typename Op>
   __device__ __forceinline__ static V lanes(V v, Op op, int from) {
@@ -223,6 +268,25 @@ struct Block {
     v = lanes(slot<V>(k)[threadIdx.x & (THREADS / 32 - 1)], op, THREADS / 64);
     if constexpr (sizeof...(rest) > 0) get(k + 1, rest...);
   }
+  template <typename V, typename Op, typename... Rest>
+  __device__ __forceinline__ void put_rank(int k, V v, Op, Rest... rest) const {
+    unsigned long long bits = 0;
+    memcpy(&bits, &v, sizeof v);
+    if (threadIdx.x < ctas) store_at(at_rank(&sh.ranks[ranks_half][k][rank], threadIdx.x), bits);
+    if constexpr (sizeof...(rest) > 0) put_rank(k + 1, rest...);
+  }
+  template <typename V>
+  __device__ __forceinline__ V of_rank(int which, int k, uint32_t r) const {
+    V v;
+    memcpy(&v, &sh.ranks[which][k][r], sizeof v);
+    return v;
+  }
+  template <typename V, typename Op, typename... Rest>
+  __device__ __forceinline__ void get_ranks(int k, V& v, Op op, Rest&&... rest) const {
+    v = of_rank<V>(ranks_half, k, 0);
+    for (uint32_t r = 1; r < ctas; ++r) v = op(v, of_rank<V>(ranks_half, k, r));
+    if constexpr (sizeof...(rest) > 0) get_ranks(k + 1, rest...);
+  }
   // reduce(value, op, value, op, ...): the values are replaced by the results.
   template <typename... Pairs>
   __device__ __forceinline__ void reduce(Pairs&&... pairs) {
@@ -231,6 +295,45 @@ struct Block {
     __syncthreads();
     get(0, pairs...);
     half ^= 1;
+    if constexpr (kCluster) {
+      put_rank(0, pairs...);
+      cluster_sync();
+      get_ranks(0, pairs...);
+      ranks_half ^= 1;
+    }
+  }
+  // Of the last reduce's value k, an int: the sum over the CTAs before this one.
+  __device__ __forceinline__ int before_rank(int k) const {
+    int sum = 0;
+    for (uint32_t r = 0; r < rank; ++r) sum += of_rank<int>(ranks_half ^ 1, k, r);
+    return sum;
+  }
+  // All threads are through with a histogram; then bins b and b + 1 of it (b even), of all CTAs.
+  __device__ __forceinline__ void meet() const {
+    if constexpr (kCluster) cluster_sync(); else __syncthreads();
+  }
+  __device__ __forceinline__ void bins(int b, bool masses, unsigned long long& w0, unsigned long long& w1) const {
+    if constexpr (kCluster) {
+      w0 = w1 = 0;
+#pragma unroll 4
+      for (uint32_t r = 0; r < ctas; ++r) {
+        const uint2 lo = load_pair_at(at_rank(&sh.bins[0][b], r));
+        w0 += lo.x;
+        w1 += lo.y;
+        if (masses) {
+          const uint2 up = load_pair_at(at_rank(&sh.bins[1][b], r));
+          w0 += (unsigned long long)up.x << 32;
+          w1 += (unsigned long long)up.y << 32;
+        }
+      }
+    } else {
+      w0 = sh.bins[0][b];
+      w1 = sh.bins[0][b + 1];
+      if (masses) {
+        w0 += (unsigned long long)sh.bins[1][b] << 32;
+        w1 += (unsigned long long)sh.bins[1][b + 1] << 32;
+      }
+    }
   }
   // Sum of the threads before this one.
   __device__ __forceinline__ unsigned long long before(unsigned long long v, unsigned long long* total) {
@@ -277,15 +380,16 @@ __device__ __forceinline__ float most_of(const Quad& x) {  // NaN is none
   return fmaxf(fmaxf(x.v[0], x.v[1]), fmaxf(x.v[2], x.v[3]));
 }
 
-template <int THREADS, bool kCached>
+template <int THREADS, bool kCached, bool kCluster>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 sample_rows_kernel(const __grid_constant__ Args A) {
   using S = Shared<THREADS>;
   constexpr int kBins = S::kBins, kListed = S::kListed;
   extern __shared__ __align__(16) float cache[];
   __shared__ S sh;
-  Block<THREADS> block{sh};
-  const int64_t row = blockIdx.x;
+  const uint32_t rank = kCluster ? cluster_rank() : 0, ctas = kCluster ? cluster_ctas() : 1;
+  Block<THREADS, kCluster> block{sh, rank, ctas};
+  const int64_t row = kCluster ? blockIdx.x / ctas : blockIdx.x;
   const int tid = threadIdx.x, C = A.cols, n = A.n;
   const float* const scores = A.scores + row * A.score_stride;
   const float* const uniforms = A.uniforms + row * A.uniform_stride;
@@ -293,12 +397,15 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   float* const probabilities = A.probabilities + row * n;
   const double T = A.temperature.at(row);
 
-  const int quads = (C + 3) / 4;
-  const auto score = [&](int i) { return kCached ? cache[i] : scores[i]; };
+  // the slice of the row that this CTA looks at
+  const int quads = (C + 3) / 4, share = kCluster ? (quads + (int)ctas - 1) / (int)ctas : quads;
+  const int q_from = kCluster ? min((int)rank * share, quads) : 0, q_to = kCluster ? min(q_from + share, quads) : quads;
+  const int i_from = kCluster ? min(4 * q_from, C) : 0, i_to = kCluster ? min(4 * q_to, C) : C;
+  const auto score = [&](int i) { return kCached ? cache[i - i_from] : scores[i]; };
   const auto score_quad = [&](int q) {
     if (!kCached) return load_quad(scores, q, C, -INFINITY);
     Quad out;
-    *reinterpret_cast<float4*>(&out) = reinterpret_cast<const float4*>(cache)[q];
+    *reinterpret_cast<float4*>(&out) = reinterpret_cast<const float4*>(cache)[q - q_from];
     return out;
   };
 
@@ -306,23 +413,24 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   // several passes later, are asked into L2 meanwhile.
   if (kCached) {
     if (((uintptr_t)scores & 15) == 0) {
-      for (int i = 4 * tid; i + 3 < C; i += 4 * THREADS) copy_async<16>(cache + i, scores + i);
-      for (int i = (C & ~3) + tid; i < C; i += THREADS) copy_async<4>(cache + i, scores + i);
+      for (int i = i_from + 4 * tid; i + 3 < i_to; i += 4 * THREADS) copy_async<16>(cache + (i - i_from), scores + i);
+      for (int i = max(i_from, i_to & ~3) + tid; i < i_to; i += THREADS) copy_async<4>(cache + (i - i_from), scores + i);
     } else {
-      for (int i = tid; i < C; i += THREADS) copy_async<4>(cache + i, scores + i);
+      for (int i = i_from + tid; i < i_to; i += THREADS) copy_async<4>(cache + (i - i_from), scores + i);
     }
     copies_commit();
-    if (C + tid < 4 * quads) cache[C + tid] = -INFINITY;
+    if (q_from < q_to && i_to + tid < 4 * q_to) cache[i_to - i_from + tid] = -INFINITY;
   }
-  for (int i = 32 * tid; i < C; i += 32 * THREADS) asm volatile("prefetch.global.L2 [%0];" ::"l"(uniforms + i));
+  for (int i = i_from + 32 * tid; i < i_to; i += 32 * THREADS) asm volatile("prefetch.global.L2 [%0];" ::"l"(uniforms + i));
   if (kCached) {
     copies_wait<0>();
     __syncthreads();
   }
+  if (kCluster) cluster_sync();  // all CTAs have begun: their shared memory may be written
   // the largest and the smallest score, and how many there are
   float best = -INFINITY, least = INFINITY;
   int some = 0;
-  for (int q = tid; q < quads; q += THREADS) {
+  for (int q = q_from + tid; q < q_to; q += THREADS) {
     const Quad x = score_quad(q);
     best = fmaxf(best, most_of(x));
 #pragma unroll
@@ -334,7 +442,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   }
   block.reduce(best, Most(), least, Least(), some, Add());
   if (some == 0 || !(T > 0.0)) {
-    for (int d = tid; d < n; d += THREADS) {
+    for (int d = tid; rank == 0 && d < n; d += THREADS) {
       indices[d] = -1;
       probabilities[d] = 0.f;
     }
@@ -358,7 +466,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   if (by_count && least < first) {  // entries that weigh nothing are no candidates
     least = INFINITY;
     some = 0;
-    for (int i = tid; i < C; i += THREADS) {
+    for (int i = i_from + tid; i < i_to; i += THREADS) {
       const float v = score(i);
       if (v >= first) {
         least = fminf(least, v);
@@ -394,10 +502,14 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       };
       __syncthreads();  // whatever the words of the union held has been read
       for (int i = tid; i < kBins; i += THREADS) sh.bins[0][i] = sh.bins[1][i] = 0;
-      if (tid == 0) sh.members = 0;
+      if (tid == 0) {
+        sh.members = 0;
+        sh.found_bin = kBins - 1;  // replaced below
+        sh.found_above = above;
+      }
       __syncthreads();
       if (masses) {
-        for (int q = tid; q < quads; q += THREADS) {
+        for (int q = q_from + tid; q < q_to; q += THREADS) {
           const Quad x = score_quad(q);
           if (!(most_of(x) >= low)) continue;
           unsigned long long w[4];
@@ -416,7 +528,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
           }
         }
       } else {
-        for (int q = tid; q < quads; q += THREADS) {
+        for (int q = q_from + tid; q < q_to; q += THREADS) {
           const Quad x = score_quad(q);
           if (!(most_of(x) >= low)) continue;
 #pragma unroll
@@ -424,11 +536,10 @@ sample_rows_kernel(const __grid_constant__ Args A) {
             if (member(x.v[e], 4 * q + e)) atomicAdd(&sh.bins[0][bin_of(x.v[e])], 1u);
         }
       }
-      __syncthreads();
+      block.meet();
       const int b0 = 2 * tid;
-      const unsigned long long w0 = sh.bins[0][b0] + ((unsigned long long)sh.bins[1][b0] << 32);
-      const unsigned long long w1 = sh.bins[0][b0 + 1] + ((unsigned long long)sh.bins[1][b0 + 1] << 32);
-      unsigned long long total;
+      unsigned long long w0, w1, total;
+      block.bins(b0, masses, w0, w1);
       const unsigned long long pre = above + block.before(w0 + w1, &total);
       if (masses && fresh) limit = p * (double)total;
       fresh = false;
@@ -441,12 +552,13 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       const int bin = sh.found_bin;
       above = sh.found_above;
       float most = -INFINITY, fewest = INFINITY;
+      int members = 0;
       // nothing of the bin lies below this: its lower end, a hundredth of its width and the rounding beyond
       const float lowest = low == high || !(per < 3e38f)
                                ? low
                                : fmaxf(low, (half * high - (bin + 1.01f) / per) / half -
                                                 4e-7f * fmaxf(fabsf(high), fabsf(low)));
-      for (int q = tid; q < quads; q += THREADS) {
+      for (int q = q_from + tid; q < q_to; q += THREADS) {
         const Quad x = score_quad(q);
         if (!(most_of(x) >= lowest)) continue;
 #pragma unroll
@@ -456,19 +568,36 @@ sample_rows_kernel(const __grid_constant__ Args A) {
           if (!(v >= lowest) || !member(v, i) || bin_of(v) != bin) continue;
           most = fmaxf(most, v);
           fewest = fminf(fewest, v);
+          if (kCluster) ++members;
           const int at = atomicAdd(&sh.members, 1);
           if (at < kListed) sh.list[at] = i;
         }
       }
-      block.reduce(most, Most(), fewest, Least());
-      const int members = sh.members;
+      if (kCluster) {
+        block.reduce(most, Most(), fewest, Least(), members, Add());
+      } else {
+        block.reduce(most, Most(), fewest, Least());
+        members = sh.members;
+      }
       if (members <= kListed) {
+        if (kCluster) {  // every CTA gets everybody's members
+          const int at = block.before_rank(2) + tid;
+          if (tid < sh.members) {
+            const int i = sh.list[tid];
+            for (uint32_t r = 0; r < ctas; ++r) {
+              store_at(at_rank(&sh.all_score[at], r), __float_as_uint(score(i)));
+              store_at(at_rank(&sh.all_index[at], r), (uint32_t)i);
+            }
+          }
+          cluster_sync();
+          if (tid < members) sh.list[tid] = sh.all_index[tid];
+        }
         static_assert(THREADS >= kListed, "a thread per ranked member");
         float mine = 0.f;
         int index = 0, rank = 0;
         if (tid < members) {
           index = sh.list[tid];
-          mine = score(index);
+          mine = kCluster ? sh.all_score[tid] : score(index);
           sh.ranked.score[tid] = mine;
         }
         __syncthreads();
@@ -528,7 +657,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
         while (from < to) {
           const int mid = from + (to - from) / 2;
           int equal = 0;
-          for (int i = tid; i <= mid; i += THREADS) {
+          for (int i = i_from + tid; i <= mid && i < i_to; i += THREADS) {
             const float v = score(i);
             equal += v == most && inside(v, i);
           }
@@ -568,7 +697,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   if (tid == 0) sh.members = 0;
   __syncthreads();
   const float lowest_kept = fmaxf(floor_score, cut);
-  for (int q = tid; q < quads; q += THREADS) {
+  for (int q = q_from + tid; q < q_to; q += THREADS) {
     const Quad x = score_quad(q);
     Quad g;
 #pragma unroll
@@ -593,13 +722,13 @@ sample_rows_kernel(const __grid_constant__ Args A) {
         }
       }
     }
-    if (kCached) reinterpret_cast<float4*>(cache)[q] = *reinterpret_cast<const float4*>(&g);
+    if (kCached) reinterpret_cast<float4*>(cache)[q - q_from] = *reinterpret_cast<const float4*>(&g);
   }
   block.reduce(total, Add(), g_most, Most(), g_least, Least(), open, Add(), odd, Or());
 
   bool listed = !(odd & 2) && (open >= n || !(odd & 1));
   if (listed && open > 0) {
-    int members = open;
+    int members = open, place = kCluster ? block.before_rank(3) : 0;  // of all; the first of this CTA's among them
     if (!filtered || open > kFew) {
       const float per = g_most > g_least ? (kBins - 1) / (g_most - g_least) : 0.f;
       const auto bounds = [&](int q) {
@@ -620,17 +749,18 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       if (tid == 0) sh.members = 0;
       if (open > n) {
         for (int i = tid; i < kBins; i += THREADS) sh.bins[0][i] = 0;
+        if (tid == 0) sh.found_bin = kBins - 1;
         __syncthreads();
-        for (int q = tid; q < quads; q += THREADS) {
+        for (int q = q_from + tid; q < q_to; q += THREADS) {
           const Quad g = bounds(q);
           if (!(most_of(g) >= g_least)) continue;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (g.v[e] >= g_least) atomicAdd(&sh.bins[0][min((int)((g_most - g.v[e]) * per), kBins - 1)], 1u);
         }
-        __syncthreads();
-        const unsigned long long c0 = sh.bins[0][2 * tid], c1 = sh.bins[0][2 * tid + 1];
-        unsigned long long all;
+        block.meet();
+        unsigned long long c0, c1, all;
+        block.bins(2 * tid, false, c0, c1);
         const unsigned long long pre = block.before(c0 + c1, &all), want = n;
         if (pre < want && pre + c0 + c1 >= want) sh.found_bin = 2 * tid + (pre + c0 < want);
         __syncthreads();
@@ -640,29 +770,43 @@ sample_rows_kernel(const __grid_constant__ Args A) {
       }
       edge -= 2.1e-6f * (fabsf(edge) + 41.f);  // what an upper bound may lie above its lower one
       __syncthreads();
-      for (int q = tid; q < quads; q += THREADS) {
+      members = 0;
+      for (int q = q_from + tid; q < q_to; q += THREADS) {
         const Quad g = bounds(q);
         if (!(most_of(g) >= edge)) continue;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (!(g.v[e] >= edge)) continue;
+          if (kCluster) ++members;
           const int at = atomicAdd(&sh.members, 1);
           if (at < kRaced) sh.list[at] = 4 * q + e;
         }
       }
-      __syncthreads();
-      members = sh.members;
+      if (kCluster) {
+        block.reduce(members, Add());
+        place = block.before_rank(0);
+      } else {
+        __syncthreads();
+        members = sh.members;
+      }
     }
     listed = members <= kRaced;
     if (listed) {
 #pragma unroll 1
-      for (int j = tid; j < members; j += THREADS) {
+      for (int j = tid; j < (kCluster ? sh.members : members); j += THREADS) {
         const int i = sh.list[j];
         const double r = race_of(scores[i], best, T, uniforms[i]) + 0.0;  // -0 as 0
         const unsigned long long bits = (unsigned long long)__double_as_longlong(r);
-        sh.race[j] = bits >> 63 ? ~bits : bits | (1ull << 63);
+        const unsigned long long image = bits >> 63 ? ~bits : bits | (1ull << 63);
+        if (kCluster) {  // the first CTA's own stay where they are, the others' come behind them
+          store_at(at_rank(&sh.race[place + j], 0), image);
+          store_at(at_rank(&sh.list[place + j], 0), (uint32_t)i);
+        } else {
+          sh.race[j] = image;
+        }
       }
-      __syncthreads();
+      block.meet();
+      if (rank != 0) return;
       if (members <= kListed) {  // ranked against each other
         if (tid < members) {
           const unsigned long long mine = sh.race[tid];
@@ -732,7 +876,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
     int at = C;
     if (more) {
 #pragma unroll 1
-      for (int i = tid; i < C; i += THREADS) {
+      for (int i = i_from + tid; i < i_to; i += THREADS) {
         if (!kept(scores[i], i)) continue;
         const double r = race_of(scores[i], best, T, uniforms[i]);
         if (!(r >= -1e300) || r > last || (r == last && i <= last_index)) continue;
@@ -749,7 +893,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
     more = at < C;
     last = most;
     last_index = at;
-    if (tid == 0) {
+    if (rank == 0 && tid == 0) {
       indices[d] = more ? at : -1;
       probabilities[d] = more ? share_of(scores[at], best, T, total) : 0.f;
     }

@@ -63,6 +63,67 @@ def test_long_rows(B, C, n):
     check(s, u, n, temperature=0.2, top_p=0.99, min_p=1e-4)
 
 
+@pytest.mark.parametrize("B,C,n", [
+    (1, 16383, 5), (1, 16384, 40), (2, 16385, 3), (27, 16387, 4), (28, 16388, 4), (74, 16390, 2), (75, 16389, 2),
+    (1, 32768, 7), (13, 32771, 4), (14, 32769, 1), (1, 99999, 33), (40, 90113, 1), (1, 327680, 5), (1, 327683, 16),
+    (6, 327681, 2), (7, 327682, 2), (1, 655361, 9), (1, 2 ** 20, 1024), (1, 2 ** 20, 1)])
+def test_rows_shared_by_a_cluster(B, C, n):
+    """Few long rows are split over the CTAs of a cluster: at and around every size where
+    the split changes, equal to the same rows drawn one CTA each, among copies of them."""
+    s, u = scores_of(B, C, C)
+    s[:, C // 2::977] = s[:, :1]  # equal scores in every slice
+    s, u = s.to(DEV), u.to(DEV)
+    copies = 75 if C <= 100000 else 3
+    for kw in (dict(temperature=0.5), dict(temperature=0.3, top_p=0.9), dict(temperature=1.0, top_k=C // 3, min_p=1e-3),
+               dict(temperature=0.2, top_k=50, top_p=0.97)):
+        got, share = maxsim.sample_candidates(s, u, n, **kw)
+        if C <= 100000:
+            want, wshare = maxsim.sample_candidates(s[:1].expand(copies, C), u[:1].expand(copies, C), n, **kw)
+            assert torch.equal(got[0], want[0]) and torch.equal(want, want[:1].expand_as(want))
+            torch.testing.assert_close(share[0], wshare[0], rtol=2.0 ** -22, atol=0)
+        check_by_sorting(s[0], u[0], got[0], share[0], **kw)
+        if B > 1:
+            check_by_sorting(s[-1], u[-1], got[-1], share[-1], **kw)
+
+
+def check_by_sorting(s, u, got, share, temperature, top_k=None, top_p=None, min_p=None):
+    """One row against the definition in 64-bit torch operations, for rows too long for
+    the oracle's loops."""
+    best, order = torch.sort(s.double(), descending=True, stable=True)
+    a = (best - best[0]) / temperature
+    keep = torch.arange(len(a), device=a.device) < (top_k or len(a))
+    w = torch.where(keep, a.exp(), 0.0)
+    if top_p:
+        keep &= w.cumsum(0) - w < top_p * w.sum()
+    if min_p:
+        keep &= a >= float(np.log(min_p))
+    race = torch.where(keep, a - torch.log(-torch.log(u.double()[order])), -INF)
+    race, place = torch.sort(race, descending=True, stable=True)
+    n = min(len(got), int(keep.sum()))
+    assert torch.equal(got[:n], order[place[:n]]) and (got[n:] == -1).all()
+    want = (a.exp() / torch.where(keep, a.exp(), 0.0).sum())[place[:n]]
+    torch.testing.assert_close(share[:n].double(), want, rtol=2.0 ** -23, atol=2.0 ** -126)
+
+
+def test_clusters_meet_every_kind_of_row():
+    """Empty rows, +inf, equal scores, uniforms at their ends, more draws than
+    candidates: the paths of a row, in a cluster."""
+    C = 16500
+    s, u = scores_of(8, C, 3)
+    s[0] = -INF
+    s[1] = float("nan")
+    s[2, 5:] = -INF
+    s[3, ::41] = INF
+    s[4] = 2.0
+    s[5] = (s[5] * 4).round() / 4
+    u[6, ::2] = 0.0
+    u[6, 1::4] = 1.0
+    u[7, ::3] = 1e-40
+    for kw in (dict(), dict(top_p=0.6), dict(top_k=700, temperature=0.1), dict(min_p=0.3, temperature=5.0)):
+        check(s, u, 12, **kw)
+    check(s[:5], u[:5], 600, top_p=0.9)
+
+
 def test_masked_rows():
     """-inf, NaN, the type's lowest value, +inf, and rows with nothing left."""
     s, u = scores_of(9, 70, 3)
