@@ -227,6 +227,24 @@ struct Affine {
   __device__ __forceinline__ float at(int c) const {
     return f32 ? static_cast<const float*>(p)[c] : widen(static_cast<const T*>(p)[c]);
   }
+  // Elements c .. c + E - 1, where p and c are on multiples of the rows' packs.
+  template <typename T, int E>
+  __device__ __forceinline__ void pack(int c, Elem<E> (&w)[kElems<E>]) const {
+    if (!f32) {
+      expand(load_pack<T, E>(static_cast<const T*>(p) + c), w);
+    } else if constexpr (E % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < E / 4; ++i) {
+        const Pack<float, 4> f = load_pack<float, 4>(static_cast<const float*>(p) + c + 4 * i);
+        w[2 * i] = pair_of(f.v[0], f.v[1]);
+        w[2 * i + 1] = pair_of(f.v[2], f.v[3]);
+      }
+    } else if constexpr (E == 2) {
+      w[0] = pair_of(at<T>(c), at<T>(c + 1));
+    } else {
+      w[0] = at<T>(c);
+    }
+  }
 };
 
 // A vector of the row's width in shared memory, as floats.  A thread's pack of
@@ -239,9 +257,25 @@ struct Wide {
   static constexpr __host__ __device__ int bytes(int dim) { return (dim + E - 1) / E * E * 4; }
   template <typename T>
   __device__ __forceinline__ void fill(const Affine& a, int dim, float none) const {
-    for (int c = threadIdx.x; c < packs * E; c += blockDim.x) {
-      const int pack = c / E, e = c % E;
-      words[((e / kPart) * packs + pack) * kPart + e % kPart] = a.p && c < dim ? a.at<T>(c) : none;
+    if (a.f32) put(static_cast<const float*>(a.p), dim, none);
+    else put(static_cast<const T*>(a.p), dim, none);
+  }
+  template <typename S>
+  __device__ __forceinline__ void put(const S* from, int dim, float none) const {
+    // Loads in flight: one after the other they took 8 us for 4096 elements.
+    constexpr int kAtOnce = 8;
+    for (int first = threadIdx.x; first < packs * E; first += kAtOnce * blockDim.x) {
+      float f[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int c = first + i * blockDim.x;
+        f[i] = from && c < dim ? widen(from[c]) : none;
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int c = first + i * blockDim.x, pack = c / E, e = c % E;
+        if (c < packs * E) words[((e / kPart) * packs + pack) * kPart + e % kPart] = f[i];
+      }
     }
   }
   __device__ __forceinline__ void get(int pack, Elem<E> (&w)[kElems<E>]) const {
@@ -919,163 +953,275 @@ grad_weight_sum_kernel(const float* __restrict__ partial, int slabs, int dim, W*
 }
 
 // ---------------------------------------------------------------------------
-// Rows of more than 4096 elements: one warp per row, several passes over it (the
-// later ones from L1 or L2), the weight's gradient by a kernel of its own.
+// Rows of more than 4096 elements: a CTA of THREADS per row, several passes over it
+// (the later ones from L1 or L2), the weight's gradient by a kernel of its own.
+//
+// HBM-bound in many rows, bound by the passes' latency in few.  us, layer norm forward / backward, one warp per
+// row and one element per load before: 4096 x 8192 bf16 38 / 86 (92 / 240; 3.5 and 2.3 TB/s), 16384 x 5120 fp32
+// 198 / 345 (311 / 817), 32 x 8192 bf16 4 / 13 (51 / 71), 1 x 2^20 bf16 106 / 356 (6332 / 7966).
 // ---------------------------------------------------------------------------
-template <typename T, int KIND>
-__global__ void __launch_bounds__(kThreads)
-forward_wide_kernel(const T* __restrict__ tokens, Rows t, Affine weight, Affine bias, T* __restrict__ out,
-                    float* __restrict__ mean, float* __restrict__ rstd, float eps) {
-  const int lane = threadIdx.x & 31;
-  const Turn<32> turn(t);
+template <int E, typename F>
+__device__ __forceinline__ void each_pack(int dim, int threads, F f) {
+#pragma unroll 4
+  for (int c = threadIdx.x * E; c < dim; c += threads * E) f(c);
+}
+
+template <typename T, int KIND, int E, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+forward_wide_kernel(const T* __restrict__ tokens, const __grid_constant__ Rows t, Affine weight, Affine bias,
+                    T* __restrict__ out, float* __restrict__ mean, float* __restrict__ rstd, float eps) {
+  using X = Elem<E>;
+  constexpr int N = kElems<E>;
+  __shared__ float words[THREADS / 8];
+  Team<THREADS> team(words);
+  const float per = 1.0f / t.dim, least = least_square(eps);
+  const Turn<THREADS> turn(t);
   Walker here;
   if (turn.begin < turn.end) here.find(t, turn.begin);
-  for (int32_t row = turn.begin + turn.mine; row < turn.end; row += Turn<32>::kRows) {
+  for (int32_t row = turn.begin; row < turn.end; ++row) {
     here.seek(t, row);
-    const T* x = tokens + here.from(t, row);
-    T* y = out + (int64_t)row * t.dim;
-    if (KIND == kLayer) {
-      float s = 0.f;
-      for (int c = lane; c < t.dim; c += 32) s += widen(x[c]);
-      const float mu = warp_sum(s) / t.dim;
-      float ss = 0.f;
-      for (int c = lane; c < t.dim; c += 32) {
-        const float d = widen(x[c]) - mu;
-        ss += d * d;
-      }
-      const float r = rsqrtf(warp_sum(ss) / t.dim + eps);
-      for (int c = lane; c < t.dim; c += 32) {
-        float h = (widen(x[c]) - mu) * r;
-        if (weight.p) h *= weight.at<T>(c);
-        if (bias.p) h += bias.at<T>(c);
-        y[c] = narrow<T>(h);
-      }
-      if (mean && lane == 0) {
+    const T* const x = tokens + here.from(t, row);
+    T* const y = out + (int64_t)row * t.dim;
+    X sum = splat<X>(0.f);
+    each_pack<E>(t.dim, THREADS, [&](int c) {
+      X f[N];
+      expand(load_pack<T, E>(x + c), f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) sum = KIND == kLayer ? add(f[i], sum) : fma(f[i], f[i], sum);
+    });
+    const float first = team.sum(total(sum));
+    if constexpr (KIND == kLayer) {
+      const float mu = first * per;
+      const X minus_mu = splat<X>(-mu);
+      sum = splat<X>(0.f);
+      each_pack<E>(t.dim, THREADS, [&](int c) {
+        X f[N];
+        expand(load_pack<T, E>(x + c), f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const X d = add(f[i], minus_mu);
+          sum = fma(d, d, sum);
+        }
+      });
+      const float r = rsqrtf(team.sum(total(sum)) * per + eps);
+      const X rr = splat<X>(r);
+      each_pack<E>(t.dim, THREADS, [&](int c) {
+        X f[N], w[N], b[N];
+        expand(load_pack<T, E>(x + c), f);
+        if (weight.p) weight.pack<T, E>(c, w);
+        if (bias.p) bias.pack<T, E>(c, b);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          f[i] = mul(add(f[i], minus_mu), rr);
+          if (weight.p) f[i] = mul(f[i], w[i]);
+          if (bias.p) f[i] = add(f[i], b[i]);
+        }
+        store_pack<T, E>(y + c, compress<T, E>(f));
+      });
+      if (mean && threadIdx.x == 0) {
         mean[row] = mu;
         rstd[row] = r;
       }
     } else {
-      float ss = 0.f, top = 0.f;
-      for (int c = lane; c < t.dim; c += 32) {
-        const float v = widen(x[c]);
-        ss += v * v;
-        top = fmaxf(top, fabsf(v));
-      }
-      ss = warp_sum(ss);
-      float inv = rsqrtf(ss);
+      float ss = first, inv = rsqrtf(ss);
       float2 by = make_float2(1.f, 1.f);
-      if (!plain_square(ss, least_square(eps))) {
-        top = warp_max(top);
+      if (!plain_square(ss, least)) {
+        float top = 0.f;
+        each_pack<E>(t.dim, THREADS, [&](int c) {
+          X f[N];
+          expand(load_pack<T, E>(x + c), f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) top = fmaxf(top, most(f[i]));
+        });
+        top = team.max(top);
         if (top > 0.f && top < INFINITY) {
           by = reciprocal_parts(top);
-          ss = 0.f;
-          for (int c = lane; c < t.dim; c += 32) {
-            const float v = widen(x[c]) * by.x * by.y;
-            ss += v * v;
-          }
-          ss = warp_sum(ss);
+          sum = splat<X>(0.f);
+          each_pack<E>(t.dim, THREADS, [&](int c) {
+            X f[N];
+            expand(load_pack<T, E>(x + c), f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const X d = mul(mul(f[i], splat<X>(by.x)), splat<X>(by.y));
+              sum = fma(d, d, sum);
+            }
+          });
+          ss = team.sum(total(sum));
         }
         const UnitScale u = unit_scale(ss, top, eps);
         inv = u.inv;
         if (!u.scaled) by = make_float2(1.f, 1.f);
       }
-      for (int c = lane; c < t.dim; c += 32) y[c] = narrow<T>(widen(x[c]) * by.x * by.y * inv);
+      each_pack<E>(t.dim, THREADS, [&](int c) {
+        X f[N];
+        expand(load_pack<T, E>(x + c), f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = mul(mul(mul(f[i], splat<X>(by.x)), splat<X>(by.y)), splat<X>(inv));
+        store_pack<T, E>(y + c, compress<T, E>(f));
+      });
     }
   }
 }
 
-// grad_tokens.  One warp per row.
-template <typename T, int KIND>
-__global__ void __launch_bounds__(kThreads)
-backward_wide_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, Rows t, Affine weight,
-                     const float* __restrict__ mean, const float* __restrict__ rstd,
+// grad_tokens.
+template <typename T, int KIND, int E, int THREADS>
+__global__ void __launch_bounds__(THREADS)
+backward_wide_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, const __grid_constant__ Rows t,
+                     Affine weight, const float* __restrict__ mean, const float* __restrict__ rstd,
                      T* __restrict__ grad_tokens, float eps) {
-  const int lane = threadIdx.x & 31;
-  const Turn<32> turn(t);
+  using X = Elem<E>;
+  constexpr int N = kElems<E>;
+  __shared__ float words[THREADS / 8];
+  Team<THREADS> team(words);
+  const float per = 1.0f / t.dim, least = least_square(eps);
+  const Turn<THREADS> turn(t);
   Walker here;
-  if (t.offsets)
-    zero_padding<T, 1>(t, grad_tokens, (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5),
-                       (int64_t)gridDim.x * (kThreads / 32), lane, 32);
+  if (t.offsets) zero_padding<T, E>(t, grad_tokens, blockIdx.x, gridDim.x, threadIdx.x, THREADS);
   if (turn.begin < turn.end) here.find(t, turn.begin);
-  for (int32_t row = turn.begin + turn.mine; row < turn.end; row += Turn<32>::kRows) {
+  for (int32_t row = turn.begin; row < turn.end; ++row) {
     here.seek(t, row);
-    const T* x = tokens + here.from(t, row);
-    const T* g = grad + (int64_t)row * t.dim;
-    T* dx = grad_tokens + here.slot(t, row) * t.dim;
-    if (KIND == kLayer) {
-      const float mu = mean[row], r = rstd[row];
-      float su = 0.f, suh = 0.f;
-      for (int c = lane; c < t.dim; c += 32) {
-        const float u = widen(g[c]) * (weight.p ? weight.at<T>(c) : 1.0f);
-        su += u;
-        suh += u * ((widen(x[c]) - mu) * r);
-      }
-      su = warp_sum(su) / t.dim;
-      suh = warp_sum(suh) / t.dim;
-      for (int c = lane; c < t.dim; c += 32) {
-        const float u = widen(g[c]) * (weight.p ? weight.at<T>(c) : 1.0f);
-        dx[c] = narrow<T>(r * (u - su - (widen(x[c]) - mu) * r * suh));
-      }
+    const T* const x = tokens + here.from(t, row);
+    const T* const g = grad + (int64_t)row * t.dim;
+    T* const dx = grad_tokens + here.slot(t, row) * t.dim;
+    const auto packs_of = [&](int c, X (&f)[N], X (&d)[N]) {
+      expand(load_pack<T, E>(x + c), f);
+      expand(load_pack<T, E>(g + c), d);
+    };
+    if constexpr (KIND == kLayer) {
+      const float r = rstd[row];
+      const X minus_mu = splat<X>(-mean[row]), rr = splat<X>(r);
+      X su = splat<X>(0.f), suh = su;
+      each_pack<E>(t.dim, THREADS, [&](int c) {
+        X f[N], u[N], w[N];
+        packs_of(c, f, u);
+        if (weight.p) weight.pack<T, E>(c, w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (weight.p) u[i] = mul(u[i], w[i]);
+          su = add(u[i], su);
+          suh = fma(u[i], mul(add(f[i], minus_mu), rr), suh);
+        }
+      });
+      const float2 both = team.sums(total(su), total(suh));
+      const X minus_u = splat<X>(-r * (both.x * per)), minus_h = splat<X>(-r * (both.y * per));
+      each_pack<E>(t.dim, THREADS, [&](int c) {
+        X f[N], u[N], w[N];
+        packs_of(c, f, u);
+        if (weight.p) weight.pack<T, E>(c, w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (weight.p) u[i] = mul(u[i], w[i]);
+          f[i] = fma(u[i], rr, fma(mul(add(f[i], minus_mu), rr), minus_h, minus_u));
+        }
+        store_pack<T, E>(dx + c, compress<T, E>(f));
+      });
     } else {
-      float ss = 0.f, xg = 0.f, top = 0.f;
-      for (int c = lane; c < t.dim; c += 32) {
-        const float v = widen(x[c]);
-        ss += v * v;
-        xg += v * widen(g[c]);
-        top = fmaxf(top, fabsf(v));
-      }
-      ss = warp_sum(ss);
-      xg = warp_sum(xg);
-      float inv = rsqrtf(ss), along = xg * inv;  // along: y . g
+      X squares = splat<X>(0.f), products = squares;
+      each_pack<E>(t.dim, THREADS, [&](int c) {
+        X f[N], d[N];
+        packs_of(c, f, d);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          squares = fma(f[i], f[i], squares);
+          products = fma(f[i], d[i], products);
+        }
+      });
+      float2 both = team.sums(total(squares), total(products));
+      float inv = rsqrtf(both.x), along = both.y * inv;  // along: y . g
       float2 by = make_float2(1.f, 1.f);
-      if (!plain_square(ss, least_square(eps))) {
-        top = warp_max(top);
+      if (!plain_square(both.x, least)) {
+        float top = 0.f;
+        each_pack<E>(t.dim, THREADS, [&](int c) {
+          X f[N];
+          expand(load_pack<T, E>(x + c), f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) top = fmaxf(top, most(f[i]));
+        });
+        top = team.max(top);
         if (top > 0.f && top < INFINITY) {
           by = reciprocal_parts(top);
-          ss = xg = 0.f;
-          for (int c = lane; c < t.dim; c += 32) {
-            const float v = widen(x[c]) * by.x * by.y;
-            ss += v * v;
-            xg += v * widen(g[c]);
-          }
-          ss = warp_sum(ss);
-          xg = warp_sum(xg);
+          squares = products = splat<X>(0.f);
+          each_pack<E>(t.dim, THREADS, [&](int c) {
+            X f[N], d[N];
+            packs_of(c, f, d);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              f[i] = mul(mul(f[i], splat<X>(by.x)), splat<X>(by.y));
+              squares = fma(f[i], f[i], squares);
+              products = fma(f[i], d[i], products);
+            }
+          });
+          both = team.sums(total(squares), total(products));
         }
-        const UnitScale u = unit_scale(ss, top, eps);
+        const UnitScale u = unit_scale(both.x, top, eps);
         inv = u.inv;
-        along = u.clamped ? 0.0f : xg * inv;
+        along = u.clamped ? 0.0f : both.y * inv;
         if (!u.scaled) by = make_float2(1.f, 1.f);
       }
-      for (int c = lane; c < t.dim; c += 32) {
-        const float h = widen(x[c]) * by.x * by.y * inv;
-        dx[c] = narrow<T>((widen(g[c]) - h * along) * inv * by.x * by.y);
-      }
+      const X minus = splat<X>(-along), ii = splat<X>(inv), bx = splat<X>(by.x), bw = splat<X>(by.y);
+      each_pack<E>(t.dim, THREADS, [&](int c) {
+        X f[N], d[N];
+        packs_of(c, f, d);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const X h = mul(mul(mul(f[i], bx), bw), ii);
+          f[i] = mul(mul(mul(fma(h, minus, d[i]), ii), bx), bw);
+        }
+        store_pack<T, E>(dx + c, compress<T, E>(f));
+      });
     }
   }
 }
 
-// Partial sums of grad_weight and grad_bias: thread = one column of one slab
-// of consecutive rows.  partial [2][slabs][dim].
-template <typename T>
+// Partial sums of grad_weight and grad_bias: a thread takes one pack of columns of one slab
+// of consecutive rows, four rows at a time.  partial [2][slabs][dim].
+template <typename T, int E>
 __global__ void __launch_bounds__(kThreads)
-grad_weight_wide_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, Rows t,
+grad_weight_wide_kernel(const T* __restrict__ grad, const T* __restrict__ tokens, const __grid_constant__ Rows t,
                         const float* __restrict__ mean, const float* __restrict__ rstd,
                         float* __restrict__ partial, int slabs) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
+  using X = Elem<E>;
+  constexpr int N = kElems<E>, kAtOnce = 4;
+  const int c = (blockIdx.x * kThreads + threadIdx.x) * E;
   const int64_t used = t.used(), share = (used + slabs - 1) / slabs;
   const int32_t begin = (int32_t)min(blockIdx.y * share, used), end = (int32_t)min(begin + share, used);
-  float dw = 0.f, db = 0.f;
   Walker here;
   if (begin < end) here.find(t, begin);
   if (c >= t.dim) return;
-  for (int32_t row = begin; row < end; ++row) {
-    here.seek(t, row);
-    const float g = widen(grad[(int64_t)row * t.dim + c]);
-    dw += g * ((widen(tokens[here.from(t, row) + c]) - mean[row]) * rstd[row]);
-    db += g;
+  X dw[N], db[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) dw[i] = db[i] = splat<X>(0.f);
+  for (int32_t row = begin; row < end; row += kAtOnce) {
+    Pack<T, E> x[kAtOnce], g[kAtOnce];
+    float mu[kAtOnce], r[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (row + k >= end) break;
+      here.seek(t, row + k);
+      x[k] = load_pack<T, E>(tokens + here.from(t, row + k) + c);
+      g[k] = load_pack<T, E>(grad + (int64_t)(row + k) * t.dim + c);
+      mu[k] = mean[row + k];
+      r[k] = rstd[row + k];
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      if (row + k >= end) break;
+      X f[N], d[N];
+      expand(x[k], f);
+      expand(g[k], d);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        dw[i] = fma(d[i], mul(add(f[i], splat<X>(-mu[k])), splat<X>(r[k])), dw[i]);
+        db[i] = add(d[i], db[i]);
+      }
+    }
   }
-  partial[(int64_t)blockIdx.y * t.dim + c] = dw;
-  partial[((int64_t)slabs + blockIdx.y) * t.dim + c] = db;
+  const Pack<float, E> pw = unpacked<E>(dw), pb = unpacked<E>(db);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    partial[(int64_t)blockIdx.y * t.dim + c + e] = pw.v[e];
+    partial[((int64_t)slabs + blockIdx.y) * t.dim + c + e] = pb.v[e];
+  }
 }
 
 }  // namespace norm

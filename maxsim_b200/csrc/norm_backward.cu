@@ -26,6 +26,12 @@ struct Backward {
     return all % bytes == 0;
   }
 
+  // Few rows in much padding: as many CTAs as its zeros keep busy.
+  void widen_for_padding(Split* split, int ctas_per_sm) const {
+    if (!t.offsets) return;
+    const int64_t most = (int64_t)sm_count() * ctas_per_sm;
+    split->grid = (unsigned)std::max<int64_t>(split->grid, std::min(most, ceil_div((int64_t)t.n_segments * t.L_max, 64)));
+  }
   template <typename T, int KIND, int E, int TEAM, int V>
   int rows() const {
     constexpr int threads = norm::kCtaThreads<TEAM>, per_sm = norm::kBackwardThreads<KIND, E, TEAM, V>;
@@ -40,28 +46,31 @@ struct Backward {
     const bool full = KIND == norm::kUnit && V * E == 16 && t.dim == TEAM * V * E;
     const int ctas = full ? std::min(512, per_sm) / threads : per_sm / threads;
     Split split = share_rows<threads, TEAM>(std::max(t.rows, 1), ctas);
-    if (t.offsets) {  // few rows in much padding: as many CTAs as its zeros keep busy
-      const int64_t most_ctas = (int64_t)sm_count() * ctas;
-      split.grid = (unsigned)std::max<int64_t>(split.grid, std::min(most_ctas, ceil_div((int64_t)t.n_segments * t.L_max, 64)));
-    }
+    widen_for_padding(&split, ctas);
     slabs = (int)split.grid;
     const int smem = fixed + (KIND == norm::kLayer ? norm::Wide<E>::bytes(t.dim) : 0);
     kern<<<split.grid, threads, smem, st>>>((const T*)grad, (const T*)tokens, split.of(t), weight, mean, rstd,
                                             (T*)grad_tokens, partial, eps);
     return launch_check("norm backward_rows_kernel");
   }
-  template <typename T, int KIND>
+  template <typename T, int KIND, int E, int THREADS>
+  int wide_rows(int ctas_per_sm) const {
+    Split split = share_rows<THREADS, THREADS>(std::max(t.rows, 1), ctas_per_sm);
+    widen_for_padding(&split, ctas_per_sm);
+    norm::backward_wide_kernel<T, KIND, E, THREADS><<<split.grid, THREADS, 0, st>>>(
+        (const T*)grad, (const T*)tokens, split.of(t), weight, mean, rstd, (T*)grad_tokens, eps);
+    return launch_check("norm backward_wide_kernel");
+  }
+  template <typename T, int KIND, int E>
   int wide() const {
     if (grad_tokens) {
-      const Split split = share_rows<norm::kThreads, 32>(std::max(t.rows, 1), 8);
-      norm::backward_wide_kernel<T, KIND><<<split.grid, norm::kThreads, 0, st>>>(
-          (const T*)grad, (const T*)tokens, split.of(t), weight, mean, rstd, (T*)grad_tokens, eps);
-      if (int rc = launch_check("norm backward_wide_kernel")) return rc;
+      const int rc = few_rows(t.rows) ? wide_rows<T, KIND, E, 1024>(1) : wide_rows<T, KIND, E, 256>(6);
+      if (rc) return rc;
     }
     if (!partial) return MAXSIM_OK;
     slabs = std::min(grad_slabs(t.rows), 64);
-    norm::grad_weight_wide_kernel<T><<<dim3((unsigned)ceil_div(t.dim, norm::kThreads), (unsigned)slabs),
-                                       norm::kThreads, 0, st>>>(
+    norm::grad_weight_wide_kernel<T, E><<<dim3((unsigned)ceil_div(t.dim, norm::kThreads * E), (unsigned)slabs),
+                                          norm::kThreads, 0, st>>>(
         (const T*)grad, (const T*)tokens, t, mean, rstd, partial, slabs);
     return launch_check("norm grad_weight_wide_kernel");
   }

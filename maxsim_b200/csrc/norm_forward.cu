@@ -38,12 +38,16 @@ struct Forward {
     kern<<<split.grid, threads, smem, st>>>((const T*)tokens, split.of(t), weight, bias, (T*)out, mean, rstd, eps);
     return launch_check(name());
   }
-  template <typename T, int KIND>
-  int wide() const {
-    const Split split = share_rows<norm::kThreads, 32>(t.rows, 8);
-    norm::forward_wide_kernel<T, KIND><<<split.grid, norm::kThreads, 0, st>>>(
+  template <typename T, int KIND, int E, int THREADS>
+  int wide_rows(int ctas_per_sm) const {
+    const Split split = share_rows<THREADS, THREADS>(t.rows, ctas_per_sm);
+    norm::forward_wide_kernel<T, KIND, E, THREADS><<<split.grid, THREADS, 0, st>>>(
         (const T*)tokens, split.of(t), weight, bias, (T*)out, mean, rstd, eps);
     return launch_check("norm forward_wide_kernel");
+  }
+  template <typename T, int KIND, int E>
+  int wide() const {
+    return few_rows(t.rows) ? wide_rows<T, KIND, E, 1024>(1) : wide_rows<T, KIND, E, 256>(6);
   }
 };
 

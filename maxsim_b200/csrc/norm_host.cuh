@@ -36,6 +36,9 @@ Split share_rows(int64_t rows, int ctas_per_sm) {
   return {(unsigned)ceil_div(rows, chunk), (int32_t)chunk};
 }
 
+// Rows of more than 4096 elements: as few as this get a CTA that fills an SM.
+bool few_rows(int64_t rows) { return rows <= 2 * sm_count(); }
+
 // The team a row gets.  Few threads with many packs cost fewer instructions a row (the
 // shuffles and the bookkeeping are shared by 32 / TEAM rows), which is what the narrow rows and the
 // forward pass are short of; the backward pass of a layer norm keeps two column sums
@@ -95,7 +98,7 @@ int by_width(const Call& call) {
     if (packs <= 1024) return call.template rows<T, KIND, E, 32, 32>();
     if (packs <= 4096) return call.template rows<T, KIND, E, norm::kWide, 32>();
   }
-  return call.template wide<T, KIND>();
+  return call.template wide<T, KIND, E>();
 }
 
 // The widest pack on whose multiples every row starts and ends.
