@@ -331,6 +331,42 @@ def test_large_offset_rows_keep_their_variance():
     check_layer(x, None, None, None, maxsim.layer_norm(x), None)
 
 
+@pytest.mark.parametrize("dim", [4097, 4098, 4104, 6000, 20001])
+@pytest.mark.parametrize("dtype,wtype", [(torch.bfloat16, torch.float32), (torch.float16, torch.float16),
+                                         (torch.float32, torch.float32)])
+@pytest.mark.parametrize("segments", [3, 160])
+def test_rows_that_take_a_cta(dim, dtype, wtype, segments):
+    """Wider than the rows that are kept on chip, few and many of them, packed, with a
+    row of zeros and rows near both ends of the type's range."""
+    L = 3
+    lengths = torch.arange(segments, dtype=torch.int32, device=DEV) % L + 1
+    x = rows_of((segments, L, dim), dtype, dim)
+    x[0, 0] = 0
+    x[1, 0] *= 2.0 ** 100 if dtype != torch.float16 else 2.0 ** 12
+    x[2, 0] *= 2.0 ** -100 if dtype != torch.float16 else 2.0 ** -16
+    x.requires_grad_(True)
+    w = rows_of((dim,), wtype, 1, 0.3, 1.0).requires_grad_(True)
+    b = rows_of((dim,), wtype, 2).requires_grad_(True)
+    T = int(lengths.sum())
+    g = rows_of((T, dim), dtype, 3)
+    valid = torch.arange(L, device=DEV)[None, :] < lengths[:, None]
+    plain = torch.ones(T, dtype=torch.bool, device=DEV)
+    plain[lengths[:1].sum()] = plain[lengths[:2].sum()] = plain[0] = False  # the three rows above
+    y, _ = maxsim.pack_unit_norm(x, lengths, total_tokens=T)
+    (dx,) = torch.autograd.grad(y, x, g)
+    assert not dx[~valid].any()
+    kept = x.detach()[valid]
+    check_unit(kept[plain], g[plain], y[plain], dx[valid][plain])
+    check_unit(kept, g, y, None)
+    with torch.no_grad():
+        x[1, 0] = x[2, 0] = x[0, 1]
+    kept = x.detach()[valid]
+    y, _ = maxsim.pack_layer_norm(x, lengths, w, b, total_tokens=T)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    assert not dx[~valid].any()
+    check_layer(kept, w, b, g, y, (dx[valid], dw, db))
+
+
 def test_empty_batches():
     for shape in ((0, 16), (3, 0, 16), (0, 4, 16)):
         x = torch.empty(shape, device=DEV, requires_grad=True)
