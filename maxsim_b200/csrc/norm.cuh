@@ -377,6 +377,9 @@ template <int KIND, int E, int TEAM, int V>
 constexpr int kBackwardThreads = KIND == kUnit ? (V * E <= 8 ? 1024 : V * E <= 16 ? 768 : 512)
                                  : V * E <= 8 || (V * E <= 16 && TEAM <= 32) ? 768
                                                                              : 512;
+// CTAs of a layer norm's backward kernel that an SM is to hold at most, whatever the instantiation (six of 128
+// threads; the host asserts it): each writes one row of partial sums, and the workspace has room for as many.
+constexpr int kSumCtas = 6;
 
 // How a row's elements get into the ring: a thread's own packs of 16 or 4 bytes; for rows of
 // 16-bit elements that start and end anywhere, the 4-byte words around them, which

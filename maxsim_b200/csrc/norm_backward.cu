@@ -4,9 +4,10 @@
 namespace maxsim {
 namespace {
 
-// Rows of the partial sums of the weight's gradient: one for each CTA of a layer norm's
-// backward kernel, at most 512 threads or four CTAs on an SM.
-int grad_slabs(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>(rows, 4 * sm_count())); }
+// Rows of the partial sums of the weight's gradient that a workspace holds: one for each CTA of a
+// layer norm's backward kernel, which never has more CTAs than there are token rows.
+int64_t grad_slabs(int64_t rows) { return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)norm::kSumCtas * sm_count())); }
+int64_t workspace_bytes_for(int64_t slabs, int64_t dim) { return slabs * dim * 2 * (int64_t)sizeof(float); }
 
 struct Backward {
   static constexpr bool kSums = true;
@@ -18,6 +19,7 @@ struct Backward {
   const float* rstd;
   void* grad_tokens;
   float* partial;  // null: no sums are wanted
+  int64_t partial_bytes;
   float eps;
   cudaStream_t st;
   mutable int slabs = 0;  // rows of `partial` that were written
@@ -26,6 +28,13 @@ struct Backward {
     return all % bytes == 0;
   }
 
+  // Before a kernel that writes `n` rows of partial sums: that there is room for them.
+  int take_slabs(int64_t n) const {
+    slabs = (int)n;
+    if (partial && workspace_bytes_for(n, t.dim) > partial_bytes)
+      return fail(MAXSIM_EWORKSPACE, "%lld rows of partial sums do not fit the workspace", (long long)n);
+    return MAXSIM_OK;
+  }
   // Few rows in much padding: as many CTAs as its zeros keep busy.
   void widen_for_padding(Split* split, int ctas_per_sm) const {
     if (!t.offsets) return;
@@ -40,6 +49,7 @@ struct Backward {
     static std::atomic<unsigned char> configured[kMaxDevices];
     constexpr int most = fixed + (KIND == norm::kLayer ? norm::Wide<E>::bytes(TEAM * V * E) : 0);
     static_assert(most <= 227 * 1024, "shared memory of a CTA");
+    static_assert(KIND != norm::kLayer || per_sm / threads <= norm::kSumCtas, "a row of the workspace for each CTA");
     if (int rc = ensure_smem(kern, most, configured)) return rc;
     // Unit rows that fill two packs of every lane keep enough in flight with two CTAs on an SM instead
     // of three (781k x 128 bf16 93 and 105 us); rows that fill them in part do not (1042k x 96: 108 and 97).
@@ -47,7 +57,7 @@ struct Backward {
     const int ctas = full ? std::min(512, per_sm) / threads : per_sm / threads;
     Split split = share_rows<threads, TEAM>(std::max(t.rows, 1), ctas);
     widen_for_padding(&split, ctas);
-    slabs = (int)split.grid;
+    if (int rc = take_slabs(split.grid)) return rc;
     const int smem = fixed + (KIND == norm::kLayer ? norm::Wide<E>::bytes(t.dim) : 0);
     kern<<<split.grid, threads, smem, st>>>((const T*)grad, (const T*)tokens, split.of(t), weight, mean, rstd,
                                             (T*)grad_tokens, partial, eps);
@@ -68,7 +78,7 @@ struct Backward {
       if (rc) return rc;
     }
     if (!partial) return MAXSIM_OK;
-    slabs = std::min(grad_slabs(t.rows), 64);
+    if (int rc = take_slabs(std::min<int64_t>(grad_slabs(t.rows), 64))) return rc;
     norm::grad_weight_wide_kernel<T, E><<<dim3((unsigned)ceil_div(t.dim, norm::kThreads * E), (unsigned)slabs),
                                           norm::kThreads, 0, st>>>(
         (const T*)grad, (const T*)tokens, t, mean, rstd, partial, slabs);
@@ -92,7 +102,7 @@ extern "C" {
 
 int64_t maxsim_b200_norm_rows_workspace(int64_t n_segments, int64_t L_max, int64_t dim) {
   if (n_segments <= 0 || L_max <= 0 || dim <= 0 || n_segments > kMaxRows / L_max) return 0;
-  return (int64_t)grad_slabs(n_segments * L_max) * dim * 2 * (int64_t)sizeof(float);
+  return workspace_bytes_for(grad_slabs(n_segments * L_max), dim);
 }
 
 int maxsim_b200_norm_rows_backward(int kind, const void* grad, const void* tokens, int64_t segment_stride,
@@ -122,7 +132,7 @@ int maxsim_b200_norm_rows_backward(int kind, const void* grad, const void* token
   if (sums && (!workspace || workspace_bytes < maxsim_b200_norm_rows_workspace(n_segments, L_max, dim)))
     return fail(MAXSIM_EWORKSPACE, "workspace missing or smaller than maxsim_b200_norm_rows_workspace says");
   const Backward call{grad, tokens, t, {weight, weight_dtype == MAXSIM_F32}, mean, rstd, grad_tokens,
-                      sums ? static_cast<float*>(workspace) : nullptr, (float)eps, st};
+                      sums ? static_cast<float*>(workspace) : nullptr, sums ? workspace_bytes : 0, (float)eps, st};
   if (int rc = launch(kind, dtype, call)) return rc;
   if (!sums) return MAXSIM_OK;
   switch (weight_dtype) {

@@ -632,3 +632,94 @@ def test_the_steps_together():
         # both sides fp32: matrix products of 192 terms, K u of the largest entry
         torch.testing.assert_close(a, want, rtol=1e-4, atol=2e-5 * float(want.abs().max()) + 1e-7, msg=lambda m: name + m)
     assert _ops.device_status() == 0
+
+
+def backward_beside_guards(x, w, g, offsets=None, guard=4 << 20):
+    """The C backward pass with a workspace of exactly the stated size between two guards:
+    ``(dx, dw, db)`` of ``x [N, L, dim]``, and whether the guards are untouched."""
+    lib, (N, L, dim) = _ops.load_library(), x.shape
+    rows = g.shape[0]
+    call = (L * dim, dim, N, L, dim, rows)
+    _, stats = _ops.norm_rows(_ops.NORM_LAYER, x, call, offsets, w, w, 1e-5, (rows, dim), True)
+    size = lib.maxsim_b200_norm_rows_workspace(N, L, dim)
+    memory = torch.full((2 * guard + size,), 0xA5, dtype=torch.uint8, device=DEV)
+    dx, dw, db = torch.empty_like(x), torch.empty(dim, dtype=w.dtype, device=DEV), torch.empty(dim, dtype=w.dtype, device=DEV)
+    rc = lib.maxsim_b200_norm_rows_backward(
+        _ops.NORM_LAYER, g.data_ptr(), x.data_ptr(), L * dim, dim, 0 if offsets is None else offsets.data_ptr(),
+        w.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr(), dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
+        memory.data_ptr() + guard, size, N, L, dim, rows, 1e-5, _ops._code(x), _ops._code(w),
+        torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, lib.maxsim_b200_last_error()
+    untouched = bool((memory[:guard] == 0xA5).all()) and bool((memory[guard + size:] == 0xA5).all())
+    return dx, dw, db, untouched
+
+
+def weights_of(dim, wtype, off):
+    return rows_of((dim + off,), wtype, 1, 0.3, 1.0)[off:]
+
+
+@pytest.mark.parametrize("dim,off", [(385, 0), (390, 0), (513, 0), (770, 0), (777, 0), (1023, 0), (768, 1)])
+@pytest.mark.parametrize("rows", [593, 888, 1185, 3000, 10000])
+def test_weight_gradients_stay_in_their_workspace(dim, off, rows):
+    """fp32 rows that no wide load divides, by their width or because the weight starts off 16
+    bytes, with more rows than the SMs hold CTAs."""
+    w = weights_of(dim, torch.float32, off)
+    x = rows_of((1, rows, dim), torch.float32, dim)
+    g = rows_of((rows, dim), torch.float32, 3)
+    dx, dw, db, untouched = backward_beside_guards(x, w, g)
+    assert untouched
+    check_layer(x[0], w, None, g, maxsim.layer_norm(x[0], w), (dx[0], dw, db))
+
+
+@pytest.mark.parametrize("dim,off", [(385, 0), (390, 0), (513, 0), (770, 0), (777, 0), (1023, 0), (768, 1)])
+def test_weight_gradients_stay_in_their_workspace_in_much_padding(dim, off):
+    """Few packed rows among 60000: the grid is widened for the zeros of the padding to as
+    many CTAs as the SMs hold, each with a row of partial sums."""
+    N, L = 15, 4000
+    w = weights_of(dim, torch.float32, off)
+    lengths = torch.arange(1, N + 1)
+    valid = (torch.arange(L)[None, :] < lengths[:, None]).to(DEV)
+    T = int(lengths.sum())
+    x = torch.full((N, L, dim), float("nan"), device=DEV)
+    kept = x[valid] = rows_of((T, dim), torch.float32, dim)
+    g = rows_of((T, dim), torch.float32, 3)
+    offsets = torch.cat([torch.zeros(1), lengths.cumsum(0)]).to(torch.int32).to(DEV)
+    dx, dw, db, untouched = backward_beside_guards(x, w, g, offsets)
+    assert untouched and not dx[~valid].any()
+    check_layer(kept, w, None, g, maxsim.layer_norm(kept, w), (dx[valid], dw, db))
+
+
+# a width for every team of threads and number of packs, for each width of a load
+PER_TEAM = {
+    torch.float32: [(32, 0), (64, 0), (128, 0), (256, 0), (512, 0), (764, 0), (1020, 0), (2044, 0), (4092, 0), (4100, 0),
+                    (31, 0), (62, 0), (95, 0), (126, 0), (255, 0), (382, 0), (1022, 0), (1025, 0), (4095, 0), (4097, 0),
+                    (128, 1), (1024, 1), (4096, 3)],
+    torch.bfloat16: [(64, 0), (128, 0), (256, 0), (512, 0), (760, 0), (1016, 0), (2040, 0), (4088, 0), (4104, 0),
+                     (30, 0), (62, 0), (126, 0), (254, 0), (382, 0), (1022, 0), (1534, 0), (4094, 0), (4098, 0),
+                     (31, 0), (63, 0), (95, 0), (127, 0), (255, 0), (383, 0), (1023, 0), (1025, 0), (4095, 0), (4097, 0),
+                     (768, 1), (768, 2), (2048, 1)],
+}
+
+
+@pytest.mark.parametrize("dtype,dim,off", [(t, *c) for t, cases in PER_TEAM.items() for c in cases])
+def test_every_team_on_a_full_gpu(dtype, dim, off):
+    """More rows than any kernel has CTAs at once (six an SM), so that CTAs and teams take several each:
+    every gradient against the oracle, weights that start off the loads' width too."""
+    rows = 1201
+    w = weights_of(dim, dtype, off)
+    x = rows_of((1, rows, dim), dtype, dim)
+    g = rows_of((rows, dim), dtype, 3)
+    dx, dw, db, untouched = backward_beside_guards(x, w, g)
+    assert untouched
+    check_layer(x[0], w, None, g, maxsim.layer_norm(x[0], w), (dx[0], dw, db))
+
+
+def test_a_workspace_that_is_too_small_is_refused():
+    x = rows_of((2000, 770), torch.float32, 0)
+    lib = _ops.load_library()
+    size = lib.maxsim_b200_norm_rows_workspace(1, 2000, 770)
+    assert size >= 6 * torch.cuda.get_device_properties(0).multi_processor_count * 770 * 8
+    args = lambda nbytes: (_ops.NORM_LAYER, x.data_ptr(), x.data_ptr(), 0, 770, 0, x.data_ptr(), x.data_ptr(),  # noqa: E731
+                           x.data_ptr(), 0, x.data_ptr(), 0, x.data_ptr(), nbytes, 1, 2000, 770, 2000, 1e-5, 0, 0, 0)
+    assert lib.maxsim_b200_norm_rows_backward(*args(size - 1)) == -4
+    assert "workspace" in lib.maxsim_b200_last_error().decode()

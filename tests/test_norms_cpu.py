@@ -189,3 +189,13 @@ def test_c_entries_refuse_without_touching_a_device():
     assert draw(n=5) == -1 and draw(rows=-1) == -1 and draw(T=0.0) == -1 and draw(stride=-1) == -1
     assert draw(cols=2 ** 20 + 1) == -2 and draw(cols=2000, n=1025) == -2
     assert draw(rows=0) == 0 and draw(n=0) == 0
+
+
+def test_workspace_has_a_row_for_every_cta():
+    """The widest grid of a layer norm's backward kernel is six CTAs on each SM (fp32 rows of 385 to
+    1024 elements that no 16-byte load divides); every CTA writes a row of sums for each of two gradients."""
+    workspace = _ops.load_library().maxsim_b200_norm_rows_workspace
+    sms = torch.cuda.get_device_properties(0).multi_processor_count if torch.cuda.is_available() else 148
+    assert workspace(1, 10000, 770) >= 6 * sms * 770 * 2 * 4
+    assert workspace(1, 600, 770) >= 600 * 770 * 2 * 4  # a CTA has a row at least
+    assert workspace(15, 4000, 777) >= 6 * sms * 777 * 2 * 4
