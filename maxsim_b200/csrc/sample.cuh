@@ -681,11 +681,14 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   // 3e-6 of its size) and the hardware's logarithm elsewhere (2^-22 of at least 0.06); the
   // outer logarithm is off by 2^-22 and what its argument is off by, a by a few 2^-24 of its size.  With
   // -4.6 < -log(-log u) < 16.7 that is less than a quarter of the 1e-6 (|sum| + 40) taken off.
-  const float inv_Tf = (float)inv_T;
+  // 1 / T is past the 32-bit range for subnormal temperatures: a product, whose first factor is a power of
+  // two.  (The second is infinite where T < 3e-77: only the best themselves are kept there, with a = 0.)
+  const bool steep = inv_T > 1e38;
+  const float scale = steep ? 0x1p126f : 1.f, inv_Tf = (float)(steep ? inv_T * 0x1p-126 : inv_T);
   const auto lower = [&](float v, float u) {
     const float t = 1.f - u;
     const float l = t < 0.0625f ? t * (1.f + t * (0.5f + t * (0.33333333f + t * 0.25f))) : -__logf(u);
-    const float g = (v == best ? 0.f : fmaxf(v - best, -3.4e38f) * inv_Tf) - __logf(l);
+    const float g = (v == best ? 0.f : fmaxf(v - best, -3.4e38f) * scale * inv_Tf) - __logf(l);
     return g - 1e-6f * (fabsf(g) + 40.f);
   };
   constexpr float kLeastUniform = 1.17549435e-38f;  // subnormal ones are raced in 64 bits
@@ -725,6 +728,9 @@ sample_rows_kernel(const __grid_constant__ Args A) {
     if (kCached) reinterpret_cast<float4*>(cache)[q - q_from] = *reinterpret_cast<const float4*>(&g);
   }
   block.reduce(total, Add(), g_most, Most(), g_least, Least(), open, Add(), odd, Or());
+  // -inf marks what is not in the race, the padding behind the row among it: whatever the
+  // bounds are, none of that is listed below
+  g_least = fmaxf(g_least, -3.4e38f);
 
   bool listed = !(odd & 2) && (open >= n || !(odd & 1));
   if (listed && open > 0) {

@@ -372,3 +372,40 @@ def test_hard_negatives_for_a_training_step():
     gq, gd = torch.autograd.grad(loss, (qa, cand))
     assert torch.isfinite(gq).all() and torch.isfinite(gd).all() and gq.abs().sum() > 0
     assert _ops.device_status() == 0
+
+
+def tiny_scores(B, C, T, seed):
+    """Scores a few subnormal temperatures apart, a tenth of them masked."""
+    g = torch.Generator().manual_seed(seed)
+    s = (torch.randn(B, C, generator=g, dtype=torch.float64) * (5 * T)).float()
+    u = torch.rand(B, C, generator=g)
+    s[torch.rand(B, C, generator=g) < 0.1] = -INF
+    s[:, 0] = 0.0
+    return s, u
+
+
+@pytest.mark.parametrize("T", [1e-38, 2e-39, 1e-39, 3e-40, 1e-42, 1e-44, 1.4e-45])
+@pytest.mark.parametrize("C", [30, 257, 1023, 4093])
+def test_subnormal_temperatures(T, C):
+    """1 / T is past the 32-bit range; what is masked, and what lies behind a row whose length is no
+    multiple of four, is never drawn."""
+    s, u = tiny_scores(5, C, T, C)
+    s[1, 2::5] = float("nan")
+    s[2, 5:] = -INF
+    s[3, C // 2:] = 1.0  # far above everything else
+    for kw in (dict(), dict(top_k=11), dict(top_k=C // 2), dict(top_p=0.9), dict(min_p=0.1), dict(top_k=C // 2, top_p=0.7)):
+        check(s, u, min(C, 25), temperature=T, **kw)
+    check(s, u, 9, temperature=torch.full((5,), T, dtype=torch.float64).float(), top_k=20)
+    pair = torch.tensor([[1e-38, 0.0]])
+    check(pair, torch.tensor([[0.5, 0.5]]), 1, temperature=T)
+    check(pair, torch.tensor([[0.5, 0.99]]), 2, temperature=T)
+
+
+@pytest.mark.parametrize("B,C", [(2, 16501), (1, 330001), (75, 41001)])
+def test_subnormal_temperatures_in_long_rows(B, C):
+    """In a cluster, and in rows that are read again instead of kept."""
+    s, u = (t.to(DEV) for t in tiny_scores(B, C, 1e-40, C))
+    for kw in (dict(), dict(top_k=C // 3), dict(top_p=0.9)):
+        got, share = maxsim.sample_candidates(s, u, 33, temperature=1e-40, **kw)
+        for row in (0, B - 1):
+            check_by_sorting(s[row], u[row], got[row], share[row], temperature=1e-40, **kw)
