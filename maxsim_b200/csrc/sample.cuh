@@ -681,14 +681,24 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   // 3e-6 of its size) and the hardware's logarithm elsewhere (2^-22 of at least 0.06); the
   // outer logarithm is off by 2^-22 and what its argument is off by, a by a few 2^-24 of its size.  With
   // -4.6 < -log(-log u) < 16.7 that is less than a quarter of the 1e-6 (|sum| + 40) taken off.
-  // 1 / T is past the 32-bit range for subnormal temperatures: a product, whose first factor is a power of
-  // two.  (The second is infinite where T < 3e-77: only the best themselves are kept there, with a = 0.)
-  const bool steep = inv_T > 1e38;
-  const float scale = steep ? 0x1p126f : 1.f, inv_Tf = (float)(steep ? inv_T * 0x1p-126 : inv_T);
+  // a is (v - best) * part times 1 / (T * part), part a power of two that keeps both inside the 32-bit range
+  // where scores are further apart than it, and where T is subnormal (there, if best * part overflows, none but the
+  // best themselves are kept, with a = 0).  A subnormal second factor is off by at most 2^-150, a by 2.4e-7.
+  const float lowest_kept = fmaxf(floor_score, cut);
+  float part = 1.f;
+  double per_part = inv_T;
+  if (inv_T > 1e38) {
+    part = 0x1p126f;
+    per_part *= 0x1p-126;
+  } else if (best < INFINITY && !(best - lowest_kept < 3.4e38f)) {
+    part = 0.5f;
+    per_part *= 2.0;
+  }
+  const float best_part = best * part, inv_Tf = (float)per_part;
   const auto lower = [&](float v, float u) {
     const float t = 1.f - u;
     const float l = t < 0.0625f ? t * (1.f + t * (0.5f + t * (0.33333333f + t * 0.25f))) : -__logf(u);
-    const float g = (v == best ? 0.f : fmaxf(v - best, -3.4e38f) * scale * inv_Tf) - __logf(l);
+    const float g = (v == best ? 0.f : fmaf(v, part, -best_part) * inv_Tf) - __logf(l);
     return g - 1e-6f * (fabsf(g) + 40.f);
   };
   constexpr float kLeastUniform = 1.17549435e-38f;  // subnormal ones are raced in 64 bits
@@ -699,7 +709,6 @@ sample_rows_kernel(const __grid_constant__ Args A) {
   __syncthreads();
   if (tid == 0) sh.members = 0;
   __syncthreads();
-  const float lowest_kept = fmaxf(floor_score, cut);
   for (int q = q_from + tid; q < q_to; q += THREADS) {
     const Quad x = score_quad(q);
     Quad g;

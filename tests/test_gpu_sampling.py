@@ -409,3 +409,37 @@ def test_subnormal_temperatures_in_long_rows(B, C):
         got, share = maxsim.sample_candidates(s, u, 33, temperature=1e-40, **kw)
         for row in (0, B - 1):
             check_by_sorting(s[row], u[row], got[row], share[row], temperature=1e-40, **kw)
+
+
+def ramp(C, dtype=torch.float64):
+    """From the lowest value of the type to the largest.  In 32 bits torch's own steps overflow:
+    +inf, -inf and NaN."""
+    top = torch.finfo(torch.float32).max
+    return torch.linspace(-top, top, C, dtype=dtype).float()
+
+
+@pytest.mark.parametrize("T", [1e35, 1e36, 3e37, 1e38, 3e38, 1e39, 1e40, 1e42, 1e45, 1e300])
+def test_scores_further_apart_than_the_type_reaches(T):
+    """Differences that are no 32-bit numbers, at temperatures that leave all scores a chance."""
+    g = torch.Generator().manual_seed(5)
+    for B, C, n in ((12, 1022, 20), (4, 4096, 60), (2, 16501, 20)):
+        for dtype in (torch.float64, torch.float32):
+            s = ramp(C, dtype).expand(B, C).clone()
+            s[1] = s[1][torch.randperm(C, generator=g)]
+            s[1, ::7] = -INF
+            u = torch.rand(B, C, generator=g)
+            for kw in (dict(), dict(top_k=C - 5), dict(top_p=0.95), dict(min_p=1e-9)):
+                check(s, u, n, temperature=T, **kw)
+
+
+def test_long_rows_further_apart_than_the_type_reaches():
+    """In a cluster, and in rows that are read again instead of kept."""
+    for B, C in ((1, 330001), (75, 41001)):
+        u = torch.rand(B, C, generator=torch.Generator(device=DEV).manual_seed(B), device=DEV)
+        s = ramp(C).to(DEV).expand(B, C)
+        assert torch.isfinite(s).all()
+        for kw in (dict(temperature=1e38), dict(temperature=1e39, top_k=C // 2), dict(temperature=1e38, top_p=0.9)):
+            got, share = maxsim.sample_candidates(s, u, 33, **kw)
+            for row in (0, B - 1):
+                check_by_sorting(s[row], u[row], got[row], share[row], **kw)
+        check(ramp(C, torch.float32)[None], u[:1].cpu(), 33, temperature=1e38)
