@@ -483,7 +483,7 @@ sample_rows_kernel(const __grid_constant__ Args A) {
     double limit = (double)k;
     float high = best, low = fmaxf(fmaxf(least, first), cut);
     if (masses) {  // below -(shift + 2) ln 2 a mass rounds to none
-      const float none = best + (-0.6931472f * (A.shift + 2)) * (float)T;
+      const float none = __double2float_rd(best_d - 0.6931471805599453 * (A.shift + 2) * T);
       low = fminf(fmaxf(low, none), best);
     }
     const auto weight = [&](float v) { return masses ? mass_of(v, best_d, per_bit, A.shift) : 1ull; };

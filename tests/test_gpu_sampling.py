@@ -443,3 +443,17 @@ def test_long_rows_further_apart_than_the_type_reaches():
             for row in (0, B - 1):
                 check_by_sorting(s[row], u[row], got[row], share[row], **kw)
         check(ramp(C, torch.float32)[None], u[:1].cpu(), 33, temperature=1e38)
+
+
+@pytest.mark.parametrize("T,step,p", [(1e-46, 1, 1 - 1e-7), (2e-45, 38, 1 - 1e-9), (1e-45, 15, 1 - 1e-9)])
+def test_masses_at_temperatures_between_the_smallest_floats(T, step, p):
+    """One best score and others `step` of the smallest float below it: the mass that top-p
+    leaves to them depends on the temperature as it was given, which is no float."""
+    g = torch.Generator().manual_seed(step)
+    s = torch.full((4, 2000), -step * 2.0 ** -149)
+    s[0, 700] = s[1, 0] = s[2, 1999] = s[3, 5] = 0.0
+    s[3, ::11] = -INF
+    u = torch.rand(4, 2000, generator=g)
+    got, _ = check(s, u, 50, temperature=T, top_p=p)
+    assert (got >= 0).all()
+    check(s, u, 50, temperature=T, top_p=p, top_k=1500)
