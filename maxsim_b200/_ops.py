@@ -18,6 +18,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import threading
 import types
 import weakref
 from pathlib import Path
@@ -458,6 +459,7 @@ GROUP_MIN_PAIRS = 2048
 _group_enabled = True
 _GROUP_CACHE = {}
 _GROUP_CACHE_LIMIT = 32
+_GROUP_LOCK = threading.Lock()  # held while the memory changes: autograd calls from threads of its own
 
 
 def set_pair_grouping(enabled: bool) -> None:
@@ -505,19 +507,22 @@ def _groups(key: torch.Tensor, ids32: torch.Tensor, n_bins: int, build: bool = T
     if not build:
         return None
     groups = group_pairs(ids32, n_bins)
-    _GROUP_CACHE.pop(id(key), None)
-    while len(_GROUP_CACHE) >= _GROUP_CACHE_LIMIT:  # the oldest only: a call needs two that stay together
-        _GROUP_CACHE.pop(next(iter(_GROUP_CACHE)))
     try:
-        _GROUP_CACHE[id(key)] = (weakref.ref(key), key._version, n_bins, groups)
+        ent = (weakref.ref(key), key._version, n_bins, groups)
     except TypeError:
-        pass
+        return groups
+    with _GROUP_LOCK:
+        _GROUP_CACHE.pop(id(key), None)
+        while len(_GROUP_CACHE) >= _GROUP_CACHE_LIMIT:  # the oldest only: a call needs two that stay together
+            _GROUP_CACHE.pop(next(iter(_GROUP_CACHE)), None)
+        _GROUP_CACHE[id(key)] = ent
     return groups
 
 
 def forget_pair_groups() -> None:
     """Drop every remembered grouping of a pair-id tensor."""
-    _GROUP_CACHE.clear()
+    with _GROUP_LOCK:
+        _GROUP_CACHE.clear()
 
 
 def _packed_args(queries, query_offsets, documents, document_offsets,
