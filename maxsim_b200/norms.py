@@ -11,7 +11,8 @@ written:
   eps) * weight + bias``;
 * :func:`unit_norm` / :func:`pack_unit_norm` -- ``x / max(|x|, eps)``.
 
-All four are differentiable once.  Statistics and sums are fp32 whatever the
+All four are differentiable once, in reverse mode (a forward-mode tangent raises
+``NotImplementedError``).  Statistics and sums are fp32 whatever the
 rows' type, every result is rounded once, and equal calls give equal bits.
 """
 
@@ -20,6 +21,7 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _ops
@@ -77,6 +79,13 @@ def _backward(ctx, grad):
 _backward_once = once_differentiable(_backward)
 
 
+def _has_tangent(*tensors) -> bool:
+    """Whether one of them carries a forward-mode tangent (which needs no gradient mode)."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside of any such differentiation
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _apply(kind, tokens, weight, bias, offsets, total, eps, lengths=None):
     """``offsets`` None: rows in, rows out."""
     if offsets is None:
@@ -88,8 +97,9 @@ def _apply(kind, tokens, weight, bias, offsets, total, eps, lengths=None):
         rows, out_shape = (src.stride(0), src.stride(1), n, L, dim, total), (total, dim)
     weight = weight if weight is None else weight.contiguous()
     bias = bias if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and (tokens.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
+    if (torch.is_grad_enabled() and (tokens.requires_grad or (weight is not None and weight.requires_grad)
+                                     or (bias is not None and bias.requires_grad))
+            or _has_tangent(tokens, weight, bias)):  # refused there: there is no forward derivative
         return _NormFn.apply(tokens, weight, bias, (kind, src, rows, offsets, eps, out_shape, lengths))
     return _ops.norm_rows(kind, src, rows, offsets, weight, bias, eps, out_shape, False, lengths)[0]
 

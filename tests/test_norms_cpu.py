@@ -199,3 +199,33 @@ def test_workspace_has_a_row_for_every_cta():
     assert workspace(1, 10000, 770) >= 6 * sms * 770 * 2 * 4
     assert workspace(1, 600, 770) >= 600 * 770 * 2 * 4  # a CTA has a row at least
     assert workspace(15, 4000, 777) >= 6 * sms * 777 * 2 * 4
+
+
+def test_forward_tangents_are_refused_not_lost(monkeypatch):
+    """A tensor with a forward-mode tangent does not require a gradient; the operators have no forward
+    derivative, and a result without a tangent would be one of zero."""
+    from torch.autograd import forward_ad
+
+    from maxsim_b200 import norms
+
+    monkeypatch.setattr(_ops, "norm_rows", lambda kind, tokens, *rest: (tokens.clone(), None))
+    x, w, b = torch.randn(3, 8), torch.ones(8), torch.zeros(8)
+    lengths = torch.tensor([2, 1], dtype=torch.int32)
+    offsets = torch.tensor([0, 2, 3], dtype=torch.int32)
+    rows = lambda x, w, b: norms._apply(_ops.NORM_LAYER, x, w, b, None, 0, 1e-5)  # noqa: E731
+    packed = lambda x, w, b: norms._apply(_ops.NORM_UNIT, x.view(1, 3, 8).expand(2, 3, 8), None, None, offsets, 3,  # noqa: E731
+                                          1e-5, lengths)
+    with forward_ad.dual_level():
+        for i, t in enumerate((x, w, b)):
+            dual = forward_ad.make_dual(t, torch.ones_like(t))
+            args = [dual if j == i else other for j, other in enumerate((x, w, b))]
+            for call in (rows, packed) if i == 0 else (rows,):
+                with pytest.raises(NotImplementedError, match="jvp|forward"):
+                    call(*args)
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="jvp|forward"):
+                    call(*args)
+                needs = [a if a is dual else a.clone().requires_grad_(True) for a in args]
+                with pytest.raises(NotImplementedError, match="jvp|forward"):
+                    call(*needs)
+        assert forward_ad.unpack_dual(rows(x, w, b)).tangent is None  # none came in
+    assert not rows(x, w, b).requires_grad
