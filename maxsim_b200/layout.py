@@ -74,6 +74,8 @@ def packed_offsets(padded: torch.Tensor, lengths: torch.Tensor, total_tokens: Op
         raise ValueError(f"lengths must have shape [N={N}]; got {tuple(lengths.shape)}")
     if lengths.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"lengths must be int32 or int64; got {lengths.dtype}")
+    if lengths.device.type != "cpu" and lengths.device != padded.device:
+        raise RuntimeError(f"lengths must be on the host or on padded's device {padded.device}; got {lengths.device}")
     if lengths.device.type == "cpu":
         if N and (int(lengths.min()) <= 0 or int(lengths.max()) > L_max):
             raise ValueError(f"lengths must be in (0, L_max={L_max}]")

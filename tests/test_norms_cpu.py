@@ -229,3 +229,17 @@ def test_forward_tangents_are_refused_not_lost(monkeypatch):
                     call(*needs)
         assert forward_ad.unpack_dual(rows(x, w, b)).tangent is None  # none came in
     assert not rows(x, w, b).requires_grad
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("total", [None, 3])
+def test_lengths_on_another_gpu_are_refused(dtype, total):
+    """Offsets made there would be an address on the wrong device: refused before any kernel."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():  # tensors that have a device and no memory
+        padded = torch.empty(3, 4, 8, device="cuda:0")
+        lengths = torch.ones(3, dtype=dtype, device="cuda:1")
+        for call in (maxsim.pack_layer_norm, maxsim.pack_unit_norm, maxsim.pack_padded):
+            with pytest.raises(RuntimeError, match="padded's device cuda:0; got cuda:1"):
+                call(padded, lengths, total_tokens=total)
