@@ -183,8 +183,8 @@ MAXSIM_API int maxsim_b200_sample_rows(const float* scores, int64_t score_stride
  * those of grad_tokens [n_segments, L_max, dim] (contiguous, zero for rows that
  * do not count), grad_weight and grad_bias [dim] that are not NULL.  grad_weight and
  * grad_bias need a workspace of maxsim_b200_norm_rows_workspace bytes on the
- * device, whose contents before and after the call do not matter; equal calls give equal
- * bits.  At most 2^31 - 4096 rows; eps >= 1e-30. */
+ * device, on a multiple of 4, whose contents before and after the call do not matter; equal
+ * calls give equal bits.  At most 2^31 - 4096 rows; eps >= 1e-30. */
 typedef enum maxsim_norm {
   MAXSIM_NORM_LAYER = 0,
   MAXSIM_NORM_UNIT = 1

@@ -131,6 +131,8 @@ int maxsim_b200_norm_rows_backward(int kind, const void* grad, const void* token
   if (kind == norm::kLayer && packed_rows > 0 && (!mean || !rstd)) return fail(MAXSIM_EINVAL, "null pointer argument");
   if (sums && (!workspace || workspace_bytes < maxsim_b200_norm_rows_workspace(n_segments, L_max, dim)))
     return fail(MAXSIM_EWORKSPACE, "workspace missing or smaller than maxsim_b200_norm_rows_workspace says");
+  if (sums && (uintptr_t)workspace % sizeof(float) != 0)
+    return fail(MAXSIM_EINVAL, "the workspace must start on a multiple of 4 bytes");
   const Backward call{grad, tokens, t, {weight, weight_dtype == MAXSIM_F32}, mean, rstd, grad_tokens,
                       sums ? static_cast<float*>(workspace) : nullptr, sums ? workspace_bytes : 0, (float)eps, st};
   if (int rc = launch(kind, dtype, call)) return rc;

@@ -243,3 +243,11 @@ def test_lengths_on_another_gpu_are_refused(dtype, total):
         for call in (maxsim.pack_layer_norm, maxsim.pack_unit_norm, maxsim.pack_padded):
             with pytest.raises(RuntimeError, match="padded's device cuda:0; got cuda:1"):
                 call(padded, lengths, total_tokens=total)
+
+
+def test_a_workspace_off_its_element_is_refused():
+    lib = _ops.load_library()
+    size = lib.maxsim_b200_norm_rows_workspace(1, 4, 8)
+    for off in (1, 2, 3):
+        rc = lib.maxsim_b200_norm_rows_backward(0, 8, 8, 32, 8, 0, 0, 8, 8, 0, 8, 0, 64 + off, size, 1, 4, 8, 4, 1e-5, 0, 0, 0)
+        assert rc == -1 and "multiple of 4" in lib.maxsim_b200_last_error().decode()
