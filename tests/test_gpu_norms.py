@@ -723,3 +723,86 @@ def test_a_workspace_that_is_too_small_is_refused():
                            x.data_ptr(), 0, x.data_ptr(), 0, x.data_ptr(), nbytes, 1, 2000, 770, 2000, 1e-5, 0, 0, 0)
     assert lib.maxsim_b200_norm_rows_backward(*args(size - 1)) == -4
     assert "workspace" in lib.maxsim_b200_last_error().decode()
+
+
+@pytest.mark.parametrize("dtype,dim,off", [(t, *c) for t, cases in PER_TEAM.items() for c in cases])
+def test_every_team_on_a_full_gpu_packed(dtype, dim, off):
+    """The same out of a padded batch with empty segments, padding that is NaN, and a gradient for
+    every padded row."""
+    N, L = 301, 8
+    lengths = torch.randint(0, L + 1, (N,), generator=torch.Generator().manual_seed(dim + off))
+    valid = (torch.arange(L)[None, :] < lengths[:, None]).to(DEV)
+    T = int(lengths.sum())
+    w = weights_of(dim, dtype, off)
+    x = torch.full((N, L, dim), float("nan"), device=DEV, dtype=dtype)
+    kept = x[valid] = rows_of((T, dim), dtype, dim)
+    g = rows_of((T, dim), dtype, 3)
+    offsets = torch.cat([torch.zeros(1), lengths.cumsum(0)]).to(torch.int32).to(DEV)
+    dx, dw, db, untouched = backward_beside_guards(x, w, g, offsets)
+    assert untouched and not dx[~valid].any()
+    y, _ = maxsim.pack_layer_norm(x, lengths.to(DEV), w, total_tokens=T)
+    check_layer(kept, w, None, g, y, (dx[valid], dw, db))
+    xa = x.requires_grad_(True)
+    y, _ = maxsim.pack_unit_norm(xa, lengths.to(DEV), total_tokens=T)
+    (dx,) = torch.autograd.grad(y, xa, g)
+    assert not dx[~valid].any()
+    check_unit(kept, g, y, dx[valid])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [1, 3, 65, 333, 777, 1025])
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+def test_weight_gradients_of_odd_rows_at_every_offset(dtype, dim, offset):
+    """16-bit rows of odd width whose first and last words reach past the tensor, into NaN: all three
+    gradients, rows as they lie and packed."""
+    N, L = 5, 6
+    base = rows_of((N * L * dim + 8,), dtype, dim)
+    base[:offset] = float("nan")
+    base[offset + N * L * dim:] = float("nan")
+    x = base[offset: offset + N * L * dim].view(N, L, dim).detach().requires_grad_(True)
+    w = rows_of((dim,), dtype, 1, 0.3, 1.0).requires_grad_(True)
+    b = rows_of((dim,), dtype, 2, 0.3, 0.0).requires_grad_(True)
+    outer = rows_of((N * L * dim + 8,), dtype, 3)
+    outer[: 1 - offset % 2] = float("nan")
+    outer[1 - offset % 2 + N * L * dim:] = float("nan")
+    g = outer[1 - offset % 2:][: N * L * dim].view(N, L, dim)
+    y = maxsim.layer_norm(x, w, b)
+    check_layer(x, w, b, g, y, torch.autograd.grad(y, (x, w, b), g))
+    lengths = torch.tensor([6, 1, 3, 2, 6])
+    valid = (torch.arange(L)[None, :] < lengths[:, None]).to(DEV)
+    gp = rows_of((18, dim), dtype, 4)
+    y, _ = maxsim.pack_layer_norm(x, lengths, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), gp)
+    assert not dx[~valid].any()
+    check_layer(x.detach()[valid], w, b, gp, y, (dx[valid], dw, db))
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, torch.bfloat16), (33, torch.float16), (770, torch.float32), (4100, torch.float32)])
+@pytest.mark.parametrize("lens,L", [([0, 3, 0, 0, 5, 0], 7), ([1] + [0] * 40, 200), ([0] * 33 + [9], 9), ([0, 0, 0], 4)])
+def test_gradients_of_empty_segments_and_much_padding(dim, dtype, lens, L):
+    x = rows_of((len(lens), L, dim), dtype, L).requires_grad_(True)
+    w = rows_of((dim,), torch.float32, 1, 0.3, 1.0).requires_grad_(True)
+    b = rows_of((dim,), torch.float32, 2, 0.3, 0.0).requires_grad_(True)
+    T, ln = sum(lens), torch.tensor(lens, device=DEV)
+    valid = torch.arange(L, device=DEV)[None, :] < ln[:, None]
+    g = rows_of((T, dim), dtype, 3)
+    y, _ = maxsim.pack_layer_norm(x, ln, w, b, total_tokens=T)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    assert not dx[~valid].any()
+    if T:
+        check_layer(x.detach()[valid], w, b, g, y, (dx[valid], dw, db))
+    else:
+        assert not dw.any() and not db.any()
+
+
+def test_forward_tangents_are_refused():
+    from torch.autograd import forward_ad
+
+    x, w = rows_of((6, 32), torch.float32, 0), rows_of((32,), torch.float32, 1)
+    with forward_ad.dual_level():
+        dual, dual_w = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(w, torch.ones_like(w))
+        for call in (lambda: maxsim.unit_norm(dual), lambda: maxsim.layer_norm(dual), lambda: maxsim.layer_norm(x, dual_w),
+                     lambda: maxsim.pack_unit_norm(dual.view(2, 3, 32), torch.tensor([1, 3]))):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(maxsim.layer_norm(x, w), maxsim.layer_norm(x.clone(), w))
