@@ -149,7 +149,9 @@ MAXSIM_API int maxsim_b200_topk_rows(const float* scores, int64_t rows, int64_t 
  * temperature (0 for the best, an infinite one included) a candidate weighs
  * exp(a_i), and one with a_i < -700 is none.  In the order score descending,
  * index ascending the filters keep the first top_k (<= 0: all), of those the
- * ones before which less than top_p of their weight lies (outside (0, 1): all),
+ * ones before which less than top_p of their weight lies (outside (0, 1): all; weights
+ * count here in steps of 2^-42 of the best for 2^20 columns, half that for half as many,
+ * down to 2^-51),
  * and the ones that weigh at least min_p of the best (outside (0, 1]: all).
  * Drawn are the n largest of a_i - log(-log(uniform_i)) among the kept, largest first, equal
  * ones by ascending index; a uniform outside [0, 1] leaves its candidate out.

@@ -353,8 +353,9 @@ __device__ __forceinline__ UnitScale unit_scale(float ss, float top, float eps) 
 //
 // HBM-bound for rows of wide packs: 5.3 to 6.2 TB/s of a copy's 6.5.  Every thread copies its own packs
 // of the next row into a ring in shared memory (cp.async) and reads back nothing but
-// what it copied itself, so the ring needs no barrier; the reductions and the store of a row run
-// under the loads of the next.
+// what it copied itself, so the ring needs no barrier (odd rows of 16-bit elements are read back by other lanes of
+// the warp and take a __syncwarp on either side); the reductions and the store of a row run under the loads of the
+// next.
 // ---------------------------------------------------------------------------
 constexpr int kWide = 128;  // threads of a team that is a CTA
 
@@ -364,8 +365,10 @@ constexpr int kCtaThreads = TEAM > 32 ? TEAM : kThreads;
 // Threads an SM is to hold at once: what the registers are cut to.  More threads are more
 // rows in flight, which past some point only hold the stores up.  Measured, 10^8 elements, us: layer norm
 // forward, 98k x 1024 bf16, 256 / 512 / 768 threads: 91 / 69 / 80; 781k x 128, 512 / 768 / 1024: 79 / 69 / 80; teams of a
-// CTA with four packs, which wait at barriers, 24k x 4096: 110 / - / 103.  Rows without wide packs are short of
-// instructions instead and take all they get.  Layer norm backward, 781k x 128 and 300k x 333 bf16, 512 / 768: 128 / 117
+// CTA with four packs, which wait at barriers, 24k x 4096, 512 / 768: 110 / 103, before the weights were staged in
+// packs (79 with 768 since).  Shared memory, which holds the weights as floats, has room for fewer of these than the
+// registers (five of six at 2304, three at 4096), and rows are split evenly over all that are launched: 48k x 2048
+// take 71, 43k x 2304 113.  Rows without wide packs are short of instructions instead and take all they get.  Layer norm backward, 781k x 128 and 300k x 333 bf16, 512 / 768: 128 / 117
 // and 293 / 258; unit rows backward, 391k x 384 bf16, 256 / 512 / 768: 108 / 103 / 115.
 template <int E, int TEAM, int V>
 constexpr int kForwardThreads = V * E <= 8                               ? 1024

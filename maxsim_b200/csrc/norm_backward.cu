@@ -51,8 +51,9 @@ struct Backward {
     static_assert(most <= 227 * 1024, "shared memory of a CTA");
     static_assert(KIND != norm::kLayer || per_sm / threads <= norm::kSumCtas, "a row of the workspace for each CTA");
     if (int rc = ensure_smem(kern, most, configured)) return rc;
-    // Unit rows that fill two packs of every lane keep enough in flight with two CTAs on an SM instead
-    // of three (781k x 128 bf16 93 and 105 us); rows that fill them in part do not (1042k x 96: 108 and 97).
+    // Unit rows that fill the 16 elements of every lane keep enough in flight with two CTAs on an SM instead
+    // of three (781k x 128 bf16 93 and 104 us, 391k x 256 93 and 104; fp32 391k x 128, 195k x 256 and 98k x 512 98
+    // and 100 each); rows that fill them in part do not (1042k x 96 bf16: 108 and 97).
     const bool full = KIND == norm::kUnit && V * E == 16 && t.dim == TEAM * V * E;
     const int ctas = full ? std::min(512, per_sm) / threads : per_sm / threads;
     Split split = share_rows<threads, TEAM>(std::max(t.rows, 1), ctas);

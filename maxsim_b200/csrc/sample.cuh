@@ -14,10 +14,13 @@
 // weights still there (the exponential race; for n = 1 the Gumbel-max form of
 // sampling).
 //
-// Which candidates come out hangs on comparisons, so a, w and the race are 64-bit
+// Which candidates come out hangs on comparisons, so a and the race are 64-bit
 // and masses are whole numbers (w * 2^shift), whose sums do not depend
-// on the order they are taken in.  (The total of the kept weights only scales the
-// probabilities: 64-bit floating point, summed in a fixed order.)
+// on the order they are taken in.  Their sum has to fit 63 bits: shift is 51 for up to 2048
+// columns and 42 for 2^20, so a mass is off by half of 2^-51 to 2^-42 of the best weight (one below
+// that is none), and by the 3e-13 of its size that the exponential's series leaves.  (The total of the
+// kept weights only scales the fp32 probabilities: 64-bit floating point, summed in a fixed order,
+// each weight good to 6e-9, a tenth of an fp32 rounding.)
 #pragma once
 
 #include <cuda_runtime.h>

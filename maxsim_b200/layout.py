@@ -192,7 +192,9 @@ def sample_candidates(scores: torch.Tensor, uniforms: torch.Tensor, n: int, *, t
 
     * ``top_k`` keeps that many;
     * ``top_p`` keeps, of those, the ones before which less than ``top_p`` of
-      their weight lies (always the best one);
+      their weight lies (always the best one).  Weights count here in steps
+      of ``2^-51`` of the best for ``C`` up to 2048, doubling with ``C`` to
+      ``2^-42``;
     * ``min_p`` keeps the ones that weigh at least ``min_p`` times the best.
 
     Each parameter is a number or a ``[B]`` tensor on the scores' device, one

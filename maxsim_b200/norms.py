@@ -154,7 +154,9 @@ def layer_norm(tokens: torch.Tensor, weight: Optional[torch.Tensor] = None,
     ``weight [D]`` and ``bias [D]`` are optional (a bias needs a weight), both
     of the tokens' type or both float32.  Differentiable with respect to all
     three; the gradients of ``weight`` and ``bias`` are summed in fp32 and have
-    their type.  Raises ``ValueError`` / ``TypeError`` for shapes and types
+    their type.  The variance is an fp32 number: rows whose squared deviations
+    from their mean add up past 3.4e38 come out as the bias, with a gradient of
+    zero.  Raises ``ValueError`` / ``TypeError`` for shapes and types
     outside this, ``RuntimeError`` for tensors that are not on one CUDA device."""
     _check("tokens", tokens, weight, bias, eps)
     return _apply(_ops.NORM_LAYER, tokens, weight, bias, None, 0, float(eps))

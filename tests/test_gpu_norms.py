@@ -795,6 +795,22 @@ def test_gradients_of_empty_segments_and_much_padding(dim, dtype, lens, L):
         assert not dw.any() and not db.any()
 
 
+def test_rows_past_the_fp32_variance():
+    """Deviations whose squares overflow: the bias and a gradient of zero, as documented, and no other row changes."""
+    for dim in (64, 333, 768, 1500, 5000):
+        x = rows_of((5, dim), torch.float32, dim)
+        w, b = rows_of((dim,), torch.float32, 1, 0.3, 1.0), rows_of((dim,), torch.float32, 2)
+        g = rows_of((5, dim), torch.float32, 3)
+        want = maxsim.layer_norm(x, w, b)
+        x[2] = rows_of((dim,), torch.float32, 4, 1e20, 0.0)
+        x.requires_grad_(True)
+        y = maxsim.layer_norm(x, w, b)
+        (dx,) = torch.autograd.grad(y, x, g)
+        others = [0, 1, 3, 4]
+        assert torch.equal(y[2], b) and not dx[2].any() and torch.equal(y[others], want[others])
+        check_layer(x.detach()[others], w, b, g[others], y[others], (dx[others], None, None))
+
+
 def test_forward_tangents_are_refused():
     from torch.autograd import forward_ad
 
